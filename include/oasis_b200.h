@@ -361,6 +361,7 @@ int oasis_dit_forward_tp(const OasisDitWeights* shard, const OasisTpArgs* a, oas
  * buffers are caller-owned so the callbacks can name them. */
 #define OASIS_DTYPE_F32 0
 #define OASIS_DTYPE_BF16 1
+#define OASIS_DTYPE_F16 2 /* paged session cache and its attention */
 typedef int (*oasis_collective_fn)(const void* send, void* recv, size_t count, int dtype, void* user,
                                    oasis_stream_t stream);
 
@@ -428,6 +429,74 @@ int oasis_peer_signal(int* flag, int value, oasis_stream_t stream);
 int oasis_peer_wait(const int* flags, int n, int skip, int target, long long timeout_ns, oasis_stream_t stream);
 int oasis_reduce_slots(void* dst, const void* staging, long long slot_stride, const void* own, int own_slot, int n,
                        long long count, int dtype, oasis_stream_t stream);
+
+/* ------------------------------------------------ paged session cache --- */
+/* Keys and values of many sequences of different lengths in pages of `page_size`
+ * tokens. A page holds every layer: pool [pages][layers][2][kv_heads][page_size]
+ * [head_dim] (keys, then values) of 2-byte elements, contiguous. Row s of `table`
+ * lists the pages of sequence s in order, lengths[s] tokens are valid, and
+ * refs[p] counts the table rows that hold page p (0: free). Entries behind a
+ * row's pages are not read. An empty cache has refs and lengths 0.
+ *
+ * The calls below change these arrays on the device, in stream order, and read
+ * nothing back, so they can be captured into a graph. Calls on one cache (and
+ * graphs that replay them) must be ordered by the caller; `workspace`
+ * (oasis_pages_workspace_size(pages, slots) bytes) belongs to the cache. What a
+ * call has to refuse on the device sets bits of *status, which stay until the
+ * caller clears them:
+ *   BAD_SEQUENCE  an index outside [0, slots), or cu decreasing
+ *   IN_USE        a fork's target that is not empty, or a target named again
+ *   NO_PAGES      the pool is full: that request, and every later one of the call
+ *                 that needs a page, changes nothing
+ *   TOO_LONG      the sequence would pass its table row
+ *   BAD_PAGE      a table entry outside the pool was met (it is skipped)
+ * Requests of one call are served in their order with the lowest free pages. */
+#define OASIS_PAGES_BAD_SEQUENCE 1
+#define OASIS_PAGES_IN_USE 2
+#define OASIS_PAGES_NO_PAGES 4
+#define OASIS_PAGES_TOO_LONG 8
+#define OASIS_PAGES_BAD_PAGE 16
+typedef struct OasisPageCache {
+  void* pool;
+  int pages, layers, kv_heads;
+  int page_size; /* a multiple of 16 up to 256 */
+  int head_dim;  /* a multiple of 8 up to 256; attention takes 64 and 128 */
+  int dtype;     /* OASIS_DTYPE_BF16 or OASIS_DTYPE_F16 */
+  int* table;    /* [slots, width] */
+  int slots, width;
+  int* lengths;  /* [slots] */
+  int* refs;     /* [pages] */
+  int* status;   /* [1] OASIS_PAGES_* bits */
+  void* workspace;
+  size_t workspace_bytes;
+} OasisPageCache;
+
+size_t oasis_pages_workspace_size(int pages, int slots);
+/* Makes room for cu[i + 1] - cu[i] more tokens behind sequence seqs[i], i < n
+ * (cu [n + 1], device), and sets start[i] to its length before, or -1 where it is
+ * refused. The sequences must differ; n <= slots. */
+int oasis_pages_reserve(const OasisPageCache* cache, const int* seqs, const int* cu, int n, int* start,
+                        oasis_stream_t stream);
+/* Writes the new tokens' keys and values of one layer: packed rows r in
+ * [cu[i], cu[i + 1]) of k and v [rows, kv_heads, head_dim] (row and head strides in
+ * elements, multiples of 8) go to positions start[i] + r - cu[i] of sequence seqs[i].
+ * Requests with start[i] < 0, rows from cu[n] on and positions behind a sequence's
+ * length are skipped. */
+int oasis_pages_write(const OasisPageCache* cache, int layer, const void* k, const void* v, long long k_row_stride,
+                      long long k_head_stride, long long v_row_stride, long long v_head_stride, const int* seqs,
+                      const int* cu, const int* start, int n, int rows, oasis_stream_t stream);
+/* Makes the empty sequences dst[i] continue src[i] (as src[i] was when the call
+ * began): whole pages are shared, the filled rows of a partial last page are copied
+ * into a page of its own. deep != 0 copies every page. */
+int oasis_pages_fork(const OasisPageCache* cache, const int* src, const int* dst, int n, int deep,
+                     oasis_stream_t stream);
+/* Empties the sequences: their pages' counts fall by one. One that is empty
+ * already, or named twice, is left. */
+int oasis_pages_free(const OasisPageCache* cache, const int* seqs, int n, oasis_stream_t stream);
+/* With n pages in use, moves the pages in use at index >= n into the free ones
+ * below it, in ascending order, and renames them in the table: [0, n) is then in
+ * use and the rest free. */
+int oasis_pages_compact(const OasisPageCache* cache, oasis_stream_t stream);
 
 /* ------------------------------------------------------------ op level --- */
 

@@ -10,6 +10,7 @@ Modules
   weights         seeded random-init weights and their device packing
   engine          native API: dit_forward, ddim_step, vae_decode, FrameEngine
   oasis_inference drop-in functions with the reference's names and call shapes
+  paged           paged session cache and the attention over it
   parallel        session data parallelism across GPUs
   build           nvcc build of the shared library
 """
@@ -21,7 +22,7 @@ __version__ = "0.1.0"
 
 def __getattr__(name):
     # engine/weights import torch CUDA plumbing lazily so CPU-only imports stay light
-    if name in ("engine", "weights", "oasis_inference", "parallel"):
+    if name in ("engine", "weights", "oasis_inference", "paged", "parallel"):
         import importlib
 
         return importlib.import_module(f"{__name__}.{name}")

@@ -128,6 +128,7 @@ class OasisTpArgs(C.Structure):
 COLLECTIVE_FN = C.CFUNCTYPE(C.c_int, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_void_p, C.c_void_p)
 OASIS_DTYPE_F32 = 0
 OASIS_DTYPE_BF16 = 1
+OASIS_DTYPE_F16 = 2
 OASIS_IPC_HANDLE_BYTES = 64
 
 
@@ -137,6 +138,12 @@ class OasisTpSpArgs(C.Structure):
                 ("xn_local", vp), ("xn", vp), ("v_local", fp), ("reduce_scatter", COLLECTIVE_FN),
                 ("all_gather", COLLECTIVE_FN), ("user", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t),
                 ("comm_stream", vp), ("chunks", C.c_int), ("reserve_sms", C.c_int)]
+
+
+class OasisPageCache(C.Structure):
+    _fields_ = [("pool", vp), ("pages", C.c_int), ("layers", C.c_int), ("kv_heads", C.c_int), ("page_size", C.c_int),
+                ("head_dim", C.c_int), ("dtype", C.c_int), ("table", vp), ("slots", C.c_int), ("width", C.c_int),
+                ("lengths", vp), ("refs", vp), ("status", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
 
 
 class OasisLayerNormArgs(C.Structure):
@@ -189,6 +196,13 @@ SIGNATURES = {
     "oasis_frame_kv_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "oasis_generate_frame_kv": (C.c_int, [C.POINTER(OasisDitWeights), C.POINTER(OasisVaeWeights),
                                           C.POINTER(OasisFrameArgs), vp]),
+    "oasis_pages_workspace_size": (C.c_size_t, [C.c_int, C.c_int]),
+    "oasis_pages_reserve": (C.c_int, [C.POINTER(OasisPageCache), vp, vp, C.c_int, vp, vp]),
+    "oasis_pages_write": (C.c_int, [C.POINTER(OasisPageCache), C.c_int, vp, vp, C.c_longlong, C.c_longlong,
+                                    C.c_longlong, C.c_longlong, vp, vp, vp, C.c_int, C.c_int, vp]),
+    "oasis_pages_fork": (C.c_int, [C.POINTER(OasisPageCache), vp, vp, C.c_int, C.c_int, vp]),
+    "oasis_pages_free": (C.c_int, [C.POINTER(OasisPageCache), vp, C.c_int, vp]),
+    "oasis_pages_compact": (C.c_int, [C.POINTER(OasisPageCache), vp]),
     "oasis_gemm": (C.c_int, [C.POINTER(OasisGemmArgs), vp]),
     "oasis_gemm_workspace_size": (C.c_size_t, [C.c_int, C.c_int, C.c_int]),
     "oasis_gemm_plan": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.POINTER(C.c_int),
