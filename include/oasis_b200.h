@@ -599,6 +599,30 @@ int oasis_attention_temporal(const void* qkv, void* out, int batch, int frames, 
 int oasis_attention_temporal_cached(const void* past_qkv, const void* cur_qkv, void* out, int batch, int past_frames,
                                     int heads, oasis_stream_t stream);
 
+/* Causal attention over whole prompts, packed: sequence i < n holds rows
+ * [cu[i], cu[i + 1]) of q, out [rows, heads, head_dim] and k, v [rows, kv_heads,
+ * head_dim]; its row r sees its rows up to r. Head h uses key head
+ * h / (heads / kv_heads). Row and head strides in elements, multiples of 8; the
+ * values of a head are contiguous and 16-byte aligned. Rows of no sequence (from
+ * cu[n] on) are not written. What a row does not see takes no part in it, whatever
+ * it holds. `longest` is a hint (the longest sequence, or an upper bound) that only
+ * chooses the kernel. The output must not overlap the inputs. Stands beside
+ * oasis_attention_temporal (one length for all, 16 x 64 heads). */
+typedef struct OasisPromptArgs {
+  const void* q; const void* k; const void* v; void* out;
+  long long q_row_stride, q_head_stride, k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+  long long out_row_stride, out_head_stride;
+  int rows;
+  const int* cu; /* [n + 1], device, non-decreasing */
+  int n, longest;
+  int heads, kv_heads;
+  int head_dim; /* 64 or 128 */
+  int dtype;    /* OASIS_DTYPE_BF16 or OASIS_DTYPE_F16 */
+  float scale;  /* 1 / sqrt(head_dim) as a rule */
+} OasisPromptArgs;
+
+int oasis_attention_prompt(const OasisPromptArgs* a, oasis_stream_t stream);
+
 /* z[r, :1024] += gate[(r / rows_per_frame) ldg + :] * (x[r, :] + bias), gate NULL =
  * plain residual. Applies the bias, adaLN gate and residual after the all-reduce of a
  * row-parallel projection (tensor parallelism: `ttnn.all_reduce` then `ttnn.add` and

@@ -146,6 +146,15 @@ class OasisPageCache(C.Structure):
                 ("lengths", vp), ("refs", vp), ("status", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
 
 
+class OasisPromptArgs(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("out", vp), ("q_row_stride", C.c_longlong),
+                ("q_head_stride", C.c_longlong), ("k_row_stride", C.c_longlong), ("k_head_stride", C.c_longlong),
+                ("v_row_stride", C.c_longlong), ("v_head_stride", C.c_longlong), ("out_row_stride", C.c_longlong),
+                ("out_head_stride", C.c_longlong), ("rows", C.c_int), ("cu", vp), ("n", C.c_int),
+                ("longest", C.c_int), ("heads", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("dtype", C.c_int), ("scale", C.c_float)]
+
+
 class OasisLayerNormArgs(C.Structure):
     _fields_ = [("x", fp), ("y", vp), ("rows_out", C.c_int), ("P", C.c_int), ("in_group", C.c_longlong),
                 ("in_off", C.c_longlong), ("frame_mul", C.c_longlong), ("frame_add", C.c_longlong),
@@ -215,6 +224,7 @@ SIGNATURES = {
     "oasis_attention_tc": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp]),
     "oasis_attention_temporal": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp]),
     "oasis_attention_temporal_cached": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
+    "oasis_attention_prompt": (C.c_int, [C.POINTER(OasisPromptArgs), vp]),
     "oasis_gated_residual": (C.c_int, [fp, fp, fp, fp, C.c_longlong, C.c_int, C.c_int, vp]),
     "oasis_post_quant": (C.c_int, [fp, fp, fp, fp, C.c_int, vp]),
 }

@@ -168,3 +168,38 @@ class PagedCache:
         if bits:
             self.status.zero_()
             raise _lib.OasisError("PagedCache", -1, "; ".join(t for b, t in STATUS.items() if bits & b))
+
+
+def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torch.Tensor, longest: int,
+                     out: torch.Tensor | None = None, scale: float | None = None, stream=None) -> torch.Tensor:
+    """Causal attention within packed sequences: rows [cu[i], cu[i + 1]) of q [rows, heads,
+    dim] and k, v [rows, kv_heads, dim] (views of packed QKV rows are fine) are one
+    sequence. dim is 64 or 128, heads a multiple of kv_heads. Rows of no sequence are
+    left as they are in `out`. `longest` (the longest sequence, or a bound) chooses the
+    kernel and nothing else."""
+    device = q.device
+    _check_device(device)
+    if q.dim() != 3 or k.dim() != 3:
+        raise ValueError("q, k and v must be [rows, heads, dim]")
+    rows, heads, dim = q.shape
+    if q.dtype not in DTYPES:
+        raise ValueError(f"q must be bfloat16 or float16, got {q.dtype}")
+    _check_rows(q, "q", q.dtype, device, None, dim)
+    _check_rows(k, "k", q.dtype, device, None, dim)
+    _check_rows(v, "v", q.dtype, device, k.shape[1], dim)
+    if k.shape[0] != rows or v.shape[0] != rows:
+        raise ValueError(f"q, k and v have {rows}, {k.shape[0]} and {v.shape[0]} rows")
+    _check_ints(cu, "cu", device)
+    if out is None:
+        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=device)
+        if stream is not None:
+            out.record_stream(stream)
+    else:
+        _check_rows(out, "out", q.dtype, device, heads, dim)
+        if out.shape[0] != rows:
+            raise ValueError(f"out has {out.shape[0]} rows, q {rows}")
+    a = _lib.OasisPromptArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_strides(q), *_strides(k),
+                             *_strides(v), *_strides(out), rows, cu.data_ptr(), max(cu.numel() - 1, 0), longest, heads,
+                             k.shape[1], dim, DTYPES[q.dtype], dim ** -0.5 if scale is None else scale)
+    _lib.call("oasis_attention_prompt", C.byref(a), _stream(stream))
+    return out

@@ -148,6 +148,12 @@ def attention_rows(q, k, v, scale=None):
     scale = 1 / math.sqrt(D) if scale is None else scale
     q, k, v = q.double(), k.double(), v.double()
     out = torch.zeros(t, H, D, dtype=torch.float64, device=q.device)
+    if n >= t > 0 and bool(torch.isfinite(k).all()) and bool(torch.isfinite(v).all()):
+        hidden = torch.arange(n, device=q.device) > torch.arange(n - t, n, device=q.device)[:, None]
+        for h in range(H):
+            x = (q[:, h] @ k[:, h // (H // K)].T * scale).masked_fill_(hidden, -math.inf)
+            out[:, h] = torch.softmax(x, -1) @ v[:, h // (H // K)]
+        return out
     for i in range(t):
         seen = n - t + i + 1
         if seen <= 0:
@@ -174,3 +180,21 @@ def attention_cached(q, pool, table, lengths, layer, seqs, scale=None):
         kv = pool[pages, layer].permute(1, 2, 0, 3, 4).reshape(2, pool.shape[3], -1, pool.shape[5])[:, :, :n]
         out.append(attention_rows(q[b : b + 1], kv[0].transpose(0, 1), kv[1].transpose(0, 1), scale))
     return torch.cat(out)
+
+
+def error_bound(want, spread, reach, keys, D, dtype):
+    """How far a kernel with 16-bit probabilities, 32-bit scores, sums and maxima may be
+    from `want` in 64 bits, element by element. `spread`: the attention over |v|;
+    `reach`: a bound of scale * sum_d |q_d k_d|; `keys`: the most keys of a row.
+    With u half a step of the type: each probability rounded once (u), the result once
+    (u); a score's sum of D products and its scaling (D + 4 roundings of 2^-24 of
+    `reach`), the maximum subtracted in the base-2 exponent (4 more), a probability
+    that is exp(score) moved by as much, in the sum and in the total (twice); the
+    exponential's own 2^-21 twice; the sums over keys (keys 2^-24 twice). `tiny`: what
+    underflows (probabilities below 2^-25 of the largest in fp16, results below the
+    smallest step)."""
+    u = torch.finfo(dtype).eps / 2
+    drift = 2 * ((D + 8) * reach * 1.4427 + 2 * keys) * 2.0 ** -24 + 2.0 ** -20
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -120
+    rel = (1 + u) * (1 + drift) * (1 + u) - 1
+    return (rel * spread + u * want.abs()) * 1.0001 + tiny * (1 + keys * (dtype == torch.float16) * 2)
