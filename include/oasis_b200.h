@@ -623,6 +623,40 @@ typedef struct OasisPromptArgs {
 
 int oasis_attention_prompt(const OasisPromptArgs* a, oasis_stream_t stream);
 
+/* Attention of one query per row over the paged cache: row b of q, out [rows, heads,
+ * head_dim] over the lengths[s] tokens of sequence s = seqs[b] in layer `layer`
+ * (after oasis_pages_write of its newest token). Head h uses key head
+ * h / (heads / kv_heads). An empty sequence gives zeros; so does an index outside
+ * the cache, which sets BAD_SEQUENCE. Pages outside the pool are left out of the sum
+ * and set BAD_PAGE.
+ * Group g is the rows [group_start[g], group_start[g + 1]) (device, non-decreasing);
+ * the first prefix_pages[g] (device) entries of its sequences' table rows have to be
+ * the same pages (as oasis_pages_fork leaves them): they are read once for the group.
+ * Rows outside all groups share nothing; groups = 0 is attention without sharing. The
+ * hints (largest group, longest prefix, most tokens behind a prefix) choose tiles and
+ * splits and nothing else; prefix_pages_hint = 0 shares nothing. The call's workspace
+ * is oasis_attention_shared_workspace_size(args) bytes (0: none) and must not be used
+ * by a call that may run at the same time. Stands beside
+ * oasis_attention_temporal_cached (one context length for all, no sharing). */
+typedef struct OasisSharedArgs {
+  const void* q; void* out;
+  long long q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements, multiples of 8 */
+  const OasisPageCache* cache;
+  int layer;
+  const int* seqs; /* [rows], device */
+  int rows, heads;
+  const int* group_start;  /* [groups + 1], device */
+  const int* prefix_pages; /* [groups], device */
+  int groups;
+  int group_rows_hint, prefix_pages_hint, own_tokens_hint;
+  float scale;
+  void* workspace;
+  size_t workspace_bytes;
+} OasisSharedArgs;
+
+size_t oasis_attention_shared_workspace_size(const OasisSharedArgs* a);
+int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream);
+
 /* z[r, :1024] += gate[(r / rows_per_frame) ldg + :] * (x[r, :] + bias), gate NULL =
  * plain residual. Applies the bias, adaLN gate and residual after the all-reduce of a
  * row-parallel projection (tensor parallelism: `ttnn.all_reduce` then `ttnn.add` and

@@ -155,6 +155,15 @@ class OasisPromptArgs(C.Structure):
                 ("dtype", C.c_int), ("scale", C.c_float)]
 
 
+class OasisSharedArgs(C.Structure):
+    _fields_ = [("q", vp), ("out", vp), ("q_row_stride", C.c_longlong), ("q_head_stride", C.c_longlong),
+                ("out_row_stride", C.c_longlong), ("out_head_stride", C.c_longlong),
+                ("cache", C.POINTER(OasisPageCache)), ("layer", C.c_int), ("seqs", vp), ("rows", C.c_int),
+                ("heads", C.c_int), ("group_start", vp), ("prefix_pages", vp), ("groups", C.c_int),
+                ("group_rows_hint", C.c_int), ("prefix_pages_hint", C.c_int), ("own_tokens_hint", C.c_int),
+                ("scale", C.c_float), ("workspace", vp), ("workspace_bytes", C.c_size_t)]
+
+
 class OasisLayerNormArgs(C.Structure):
     _fields_ = [("x", fp), ("y", vp), ("rows_out", C.c_int), ("P", C.c_int), ("in_group", C.c_longlong),
                 ("in_off", C.c_longlong), ("frame_mul", C.c_longlong), ("frame_add", C.c_longlong),
@@ -225,6 +234,8 @@ SIGNATURES = {
     "oasis_attention_temporal": (C.c_int, [vp, vp, C.c_int, C.c_int, C.c_int, vp]),
     "oasis_attention_temporal_cached": (C.c_int, [vp, vp, vp, C.c_int, C.c_int, C.c_int, vp]),
     "oasis_attention_prompt": (C.c_int, [C.POINTER(OasisPromptArgs), vp]),
+    "oasis_attention_shared_workspace_size": (C.c_size_t, [C.POINTER(OasisSharedArgs)]),
+    "oasis_attention_shared": (C.c_int, [C.POINTER(OasisSharedArgs), vp]),
     "oasis_gated_residual": (C.c_int, [fp, fp, fp, fp, C.c_longlong, C.c_int, C.c_int, vp]),
     "oasis_post_quant": (C.c_int, [fp, fp, fp, fp, C.c_int, vp]),
 }

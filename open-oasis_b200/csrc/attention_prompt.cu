@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(PromptParams 
     }
     __syncthreads();  // the tile may be overwritten
   }
-  cp_async_wait<0>();  // a tile without keys has only Q in flight
+  cp_async_wait_all();  // a tile without keys has only Q in flight
 #pragma unroll
   for (int w = 1; w < 4; w <<= 1) {
     la += __shfl_xor_sync(0xffffffffu, la, w);

@@ -15,6 +15,8 @@ __device__ __forceinline__ void cp_async16(void* smem, const void* gmem, bool va
                : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Every copy of this thread, committed to a group or not.
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
@@ -87,9 +89,9 @@ __device__ __forceinline__ bool finite_f(float x) { return fabsf(x) <= 3.4028234
 // of the j-th visible key or null for one to skip. The tiled kernels multiply a
 // masked probability of zero with whatever the masked value row holds, which is
 // wrong where that is an infinity or NaN; rows whose result is not finite are done
-// again here, where only visible keys take part.
+// again here, where only visible keys take part. Returns whether any key did.
 template <typename T, int D, typename Key, typename Val>
-__device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long keys, Key key, Val val,
+__device__ __noinline__ bool row_by_keys(const T* q, float scale_log2, long long keys, Key key, Val val,
                                          float (&o)[D / 32], float& m, float& l) {
   constexpr int DV = D / 32;
   const int lane = threadIdx.x & 31;
@@ -100,9 +102,11 @@ __device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long
     qv[d] = x.x;
     qv[d + 1] = x.y;
   }
+  bool any = false;
   for (long long j = 0; j < keys; ++j) {
     const T* kp = key(j);
     if (!kp) continue;
+    any = true;
     float s = 0.f;
 #pragma unroll
     for (int d = 0; d < DV; d += 2) {
@@ -124,6 +128,7 @@ __device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long
     }
     m = mn;
   }
+  return any;
 }
 
 }  // namespace oasis

@@ -1,0 +1,692 @@
+// Attention of one query per row over the paged cache, for batches whose rows share a
+// prefix. Row b, head h, sequence s = seqs[b] with length t:
+//   o = sum_{j < t} exp(x_j - m) v_j / sum_{j < t} exp(x_j - m),  x_j = scale q . k_j,  m = max x_j
+// Keys split into ranges; a range gives (m_r, l_r, o~_r) with l_r and o~_r relative to
+// its own maximum, and ranges join as m = max m_r, l = sum l_r e^(m_r - m),
+// o = sum e^(m_r - m) o~_r / l.
+//
+// shared_prefix_kernel: the keys that a group's rows have in common, read once for all
+// of them: 64 (row, head) queries of one key head per block, 64 keys a step, mma.sync.
+// shared_own_kernel: each row's keys behind the prefix: a warp per (row, key head,
+// split), 16 keys a step, the heads of a group as the 16 rows of a fragment. Bound by
+// reading the keys and values once. With one split it joins the prefix ranges too and
+// writes the result; otherwise shared_join_kernel does.
+#include "../../include/oasis_b200.h"
+#include "attention_rows.cuh"
+#include "gemm.cuh"
+#include "pages.cuh"
+#include "status.h"
+
+namespace oasis {
+namespace {
+
+constexpr int kUnit = 16;           // keys of a step of a warp: always inside one page
+constexpr int kPrefixRows = 64;     // (row, head) queries of a block
+constexpr int kPrefixKeys = 64;     // keys of a step
+constexpr int kThreads = 128;
+constexpr int kOwnWarps = 4;
+constexpr int kMostSplits = 64;
+
+struct SharedParams {
+  PageGeometry g;
+  const void *q, *pool;
+  void* out;
+  long long q_row, q_head, o_row, o_head;
+  const int *table, *lengths, *seqs, *group_start, *prefix_pages;
+  int* status;
+  float* part_o;   // [rows heads][splits][D]
+  float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
+  int rows, groups, heads, per, layer;  // per: heads of a key head
+  int prefix_splits, own_splits, tiles, head_tiles;
+  float scale_log2;
+};
+
+// Length of row b's sequence, 0 where there is none; `s` its slot.
+__device__ __forceinline__ int row_length(const SharedParams& p, int b, int* s) {
+  const int x = p.seqs[b];
+  *s = x;
+  if (x < 0 || x >= p.g.slots) return 0;
+  return held_tokens(p.lengths[x], p.g.page_size, p.g.width);
+}
+
+// Group of row b, by the whole warp: the last one that starts at or before b; -1
+// where b lies outside of them.
+__device__ __forceinline__ int row_group(const SharedParams& p, int b) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = p.groups;  // the answer is in [lo, lo + n)
+  if (n < 1 || p.group_start[0] > b || p.group_start[p.groups] <= b) return -1;
+  while (n > 1) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const bool ok = i < n && p.group_start[lo + i] <= b;
+    const int c = 32 - __clz(__ballot_sync(0xffffffffu, ok) | 1u);  // probes that hold: a run from lane 0
+    lo += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+  return lo;
+}
+
+__device__ __forceinline__ int group_tokens(const SharedParams& p, int group) {
+  return group < 0 ? 0 : held_tokens(p.prefix_pages[group], 1, p.g.width) * p.g.page_size;
+}
+
+template <int D>
+constexpr int prefix_smem() {
+  return (kPrefixRows + 4 * kPrefixKeys) * D * 2;
+}
+template <int D>
+constexpr int own_smem() {
+  return kOwnWarps * 4 * kUnit * D * 2;
+}
+
+// One running-softmax step of a warp: 16 queries x 16 keys. `see(e, key)` masks; x
+// holds the scores of key tiles 0 and 1 in fragment order and becomes P.
+struct Running {
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+};
+
+template <typename T>
+__device__ __forceinline__ void softmax_step(float (&x)[2][4], Running& r, float& fa, float& fb, uint32_t (&pa)[4]) {
+  float na = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
+  float nb = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+#pragma unroll
+  for (int w = 1; w < 4; w <<= 1) {
+    na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, w));
+    nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, w));
+  }
+  na = fmaxf(na, r.ma);
+  nb = fmaxf(nb, r.mb);
+  const float sa = softmax_shift(na), sb = softmax_shift(nb);
+  fa = ex2_approx(r.ma - sa);
+  fb = ex2_approx(r.mb - sb);
+  r.ma = na;
+  r.mb = nb;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    x[t][0] = ex2_approx(x[t][0] - sa);
+    x[t][1] = ex2_approx(x[t][1] - sa);
+    x[t][2] = ex2_approx(x[t][2] - sb);
+    x[t][3] = ex2_approx(x[t][3] - sb);
+  }
+  r.la = r.la * fa + ((x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));  // this lane's share
+  r.lb = r.lb * fb + ((x[0][2] + x[0][3]) + (x[1][2] + x[1][3]));
+  // P as the 16-bit operand: the one rounding inside the sum
+  pa[0] = Elem<T>::pack(x[0][0], x[0][1]);
+  pa[1] = Elem<T>::pack(x[0][2], x[0][3]);
+  pa[2] = Elem<T>::pack(x[1][0], x[1][1]);
+  pa[3] = Elem<T>::pack(x[1][2], x[1][3]);
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void scores(const uint8_t* sk, int row0, const uint32_t (&qa)[D / 16][4], float (&x)[2][4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    uint32_t b[4];
+    ldsm_x4(b, sk + tile_at<D>(row0 + (lane & 7) + ((lane >> 4) << 3), s * 2 + ((lane >> 3) & 1)));
+    Elem<T>::mma(x[0], qa[s], b[0], b[1]);
+    Elem<T>::mma(x[1], qa[s], b[2], b[3]);
+  }
+}
+
+template <typename T, int D>
+__device__ __forceinline__ void add_values(const uint8_t* sv, int row0, const uint32_t (&pa)[4], float fa, float fb,
+                                           float (&o)[D / 8][4]) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int t = 0; t < D / 8; t += 2) {
+    uint32_t b[4];
+    ldsm_x4_t(b, sv + tile_at<D>(row0 + (lane & 15), t + (lane >> 4)));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      o[t + u][0] *= fa;
+      o[t + u][1] *= fa;
+      o[t + u][2] *= fb;
+      o[t + u][3] *= fb;
+      Elem<T>::mma(o[t + u], pa, b[2 * u], b[2 * u + 1]);
+    }
+  }
+}
+
+__device__ __forceinline__ void join_lanes(Running& r) {
+#pragma unroll
+  for (int w = 1; w < 4; w <<= 1) {
+    r.la += __shfl_xor_sync(0xffffffffu, r.la, w);
+    r.lb += __shfl_xor_sync(0xffffffffu, r.lb, w);
+  }
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p) {
+  constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kPrefixKeys * D * 2;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int limit[kPrefixRows];  // keys that a query sees; -1: no query
+  __shared__ int lead_len[4], lead_row[4];
+  __shared__ int unit_ok[2][4];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int x = blockIdx.x;
+  const int tile = x % p.tiles;
+  x /= p.tiles;
+  const int split = x % p.prefix_splits;
+  x /= p.prefix_splits;
+  const int kvh = x % p.g.kv_heads, group = x / p.g.kv_heads;
+  const int b0 = max(0, p.group_start[group]), b1 = min(p.rows, p.group_start[group + 1]);
+  const int P = p.g.page_size;
+  const int tokens = group_tokens(p, group);
+  const long long queries = (long long)max(0, b1 - b0) * p.per;
+  if ((long long)tile * kPrefixRows >= queries) return;
+
+  // The prefix is read through the table row of the longest sequence (the first of
+  // them): a shorter one need not have all of its pages.
+  int len = -1, row = b1;
+  for (int b = b0 + tid; b < b1; b += kThreads) {
+    int s;
+    const int t = row_length(p, b, &s);
+    if (t > len) {
+      len = t;
+      row = b;
+    }
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) {
+    const int l2 = __shfl_xor_sync(0xffffffffu, len, w), r2 = __shfl_xor_sync(0xffffffffu, row, w);
+    if (l2 > len || (l2 == len && r2 < row)) {
+      len = l2;
+      row = r2;
+    }
+  }
+  if (lane == 0) {
+    lead_len[warp] = len;
+    lead_row[warp] = row;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 4; ++w)
+    if (lead_len[w] > len || (lead_len[w] == len && lead_row[w] < row)) {
+      len = lead_len[w];
+      row = lead_row[w];
+    }
+  const int common = min(tokens, len);  // whole and valid pages but for the last
+  const int* lead = p.table + (long long)(len > 0 ? p.seqs[row] : 0) * p.g.width;
+  const int units = (max(common, 0) + kUnit - 1) / kUnit;
+  const int u0 = (int)((long long)units * split / p.prefix_splits), u1 = (int)((long long)units * (split + 1) / p.prefix_splits);
+  const int steps = (u1 - u0 + 3) / 4;
+
+  for (long long m0 = (long long)tile * kPrefixRows; m0 < queries; m0 += (long long)p.tiles * kPrefixRows) {
+    __syncthreads();
+    if (tid < kPrefixRows) {
+      const long long m = m0 + tid;
+      int lim = -1, s;
+      if (m < queries) lim = min(common, row_length(p, b0 + (int)(m / p.per), &s));
+      limit[tid] = lim;
+    }
+    const T* q = static_cast<const T*>(p.q);
+    for (int i = tid; i < kPrefixRows * CH; i += kThreads) {
+      const int r = i / CH, c = i % CH;
+      const bool ok = m0 + r < queries;
+      const long long m = ok ? m0 + r : m0;
+      const long long b = b0 + m / p.per;
+      const int h = kvh * p.per + (int)(m % p.per);
+      cp_async16(sm + tile_at<D>(r, c), q + b * p.q_row + h * p.q_head + c * 8, ok);
+    }
+    auto load = [&](int j) {
+      uint8_t* kd = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+      const uint4* pool = static_cast<const uint4*>(p.pool);
+      for (int i = tid; i < kPrefixKeys * CH; i += kThreads) {
+        const int r = i / CH, c = i % CH;
+        const int u = u0 + j * 4 + r / kUnit;
+        const int t = u * kUnit;
+        const int page = u < u1 ? lead[t / P] : -1;
+        const bool ok = page_ok(page, p.g.pages);
+        const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P + r % kUnit) * CH + c;
+        cp_async16(kd + tile_at<D>(r, c), pool + at, ok);
+        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + p.g.kv_heads * tile_vectors(p.g), ok);
+        if (c == 0 && r % kUnit == 0) {
+          unit_ok[j & 1][r / kUnit] = ok;
+          if (!ok && u < u1) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+        }
+      }
+      cp_async_commit();
+    };
+    if (steps > 0) load(0);
+    const int wr = warp * 16, ra = wr + (lane >> 2);
+    uint32_t qa[KS][4];
+    float o[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+    Running run;
+    int lim_a = -1, lim_b = -1;
+    for (int j = 0; j < steps; ++j) {
+      if (j + 1 < steps) {
+        load(j + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncthreads();
+      if (j == 0) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
+        lim_a = limit[ra];
+        lim_b = limit[ra + 8];
+      }
+      const uint8_t* sk = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (!unit_ok[j & 1][h]) continue;
+        const int kb = (u0 + j * 4 + h) * kUnit;
+        float s[2][4] = {};
+        scores<T, D>(sk, h * kUnit, qa, s);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = kb + t * 8 + (lane & 3) * 2 + (e & 1);
+            s[t][e] = key < (e < 2 ? lim_a : lim_b) ? s[t][e] * p.scale_log2 : -INFINITY;
+          }
+        float fa, fb;
+        uint32_t pa[4];
+        softmax_step<T>(s, run, fa, fb, pa);
+        add_values<T, D>(sk + TILE, h * kUnit, pa, fa, fb, o);
+      }
+      __syncthreads();
+    }
+    cp_async_wait_all();  // a range without keys has only Q in flight
+    join_lanes(run);
+    const int splits = p.prefix_splits + p.own_splits;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const long long m = m0 + ra + half * 8;
+      if (m >= queries) continue;
+      const long long b = b0 + m / p.per;
+      const int h = kvh * p.per + (int)(m % p.per);
+      const long long slot = (b * p.heads + h) * splits + split;
+      const float mm = half ? run.mb : run.ma, ll = half ? run.lb : run.la;
+      if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm, ll);
+      if (mm == -INFINITY && ll == 0.f) continue;  // nothing in this range: its sums are not read
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<float2*>(p.part_o + slot * D + t * 8 + (lane & 3) * 2) =
+            make_float2(o[t][2 * half], o[t][2 * half + 1]);
+    }
+  }
+}
+
+// A row's result where the joined ranges are not finite: key by key, so that masked
+// places and the formula's own NaN come out as they should. Whole warp.
+template <typename T, int D>
+__device__ __noinline__ void row_again(const SharedParams& p, int b, int h) {
+  int s;
+  const int len = row_length(p, b, &s), lane = threadIdx.x & 31, P = p.g.page_size;
+  const int* table = p.table + (long long)s * p.g.width;
+  const T* pool = static_cast<const T*>(p.pool);
+  const int kvh = h / p.per;
+  auto at = [&](long long j, int which) -> const T* {
+    const int page = table[j / P];
+    if (!page_ok(page, p.g.pages)) return nullptr;
+    return pool + (tile_offset(p.g, page, p.layer, which, kvh) + (j % P) * (D / 8)) * 8;
+  };
+  float acc[D / 32] = {}, m = -INFINITY, l = 0.f;
+  const bool any = row_by_keys<T, D>(
+      static_cast<const T*>(p.q) + b * p.q_row + h * p.q_head, p.scale_log2, len,
+      [&](long long j) { return at(j, 0); }, [&](long long j) { return at(j, 1); }, acc, m, l);
+  if (!any) l = 1.f;  // no page of it lies in the pool: zeros
+  T* out = static_cast<T*>(p.out) + b * p.o_row + h * p.o_head;
+#pragma unroll
+  for (int d = 0; d < D / 32; d += 2)
+    *reinterpret_cast<uint32_t*>(out + lane * (D / 32) + d) = Elem<T>::pack(acc[d] / l, acc[d + 1] / l);
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams p) {
+  constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kUnit * D * 2;
+  extern __shared__ __align__(128) uint8_t sm[];
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint8_t* ring = sm + warp * 4 * TILE;
+  const long long item = (long long)blockIdx.x * kOwnWarps + warp;
+  long long x = item;
+  const int split = (int)(x % p.own_splits);
+  x /= p.own_splits;
+  const int ht = (int)(x % p.head_tiles);
+  x /= p.head_tiles;
+  const int kvh = (int)(x % p.g.kv_heads);
+  const int b = (int)(x / p.g.kv_heads);
+  if (b >= p.rows) return;  // whole warps; no block-wide barrier follows
+  int s;
+  const int len = row_length(p, b, &s), P = p.g.page_size;
+  if (s < 0 || s >= p.g.slots) {
+    if (lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);
+    s = 0;
+  }
+  const int group = p.prefix_splits ? row_group(p, b) : -1;
+  const int begin = group_tokens(p, group);
+  const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
+  const int u0 = (int)((long long)units * split / p.own_splits), u1 = (int)((long long)units * (split + 1) / p.own_splits);
+  const int* table = p.table + (long long)s * p.g.width;
+  const uint4* pool = static_cast<const uint4*>(p.pool);
+  const int nh = min(16, p.per - ht * 16), h0 = kvh * p.per + ht * 16;  // heads of this fragment
+
+  unsigned ok_bits = 0;  // of the two units in flight
+  auto load = [&](int u) {
+    uint8_t* kd = ring + (u & 1) * 2 * TILE;
+    const int t = begin + u * kUnit;
+    const int page = table[t / P];
+    const bool ok = page_ok(page, p.g.pages);
+    ok_bits = (ok_bits & ~(1u << (u & 1))) | ((unsigned)ok << (u & 1));
+    if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+    const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P) * CH;
+    const long long to_v = p.g.kv_heads * tile_vectors(p.g);
+#pragma unroll
+    for (int i = 0; i < kUnit * CH / 32; ++i) {
+      const int y = i * 32 + lane, r = y / CH, c = y % CH;
+      const bool in = ok && t + r < len;  // rows behind the sequence hold anything: zero instead
+      cp_async16(kd + tile_at<D>(r, c), pool + at + y, in);
+      cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + to_v + y, in);
+    }
+    cp_async_commit();
+  };
+  if (u0 < u1) load(u0);
+
+  const int ra = lane >> 2;
+  const T* q = static_cast<const T*>(p.q) + b * p.q_row + h0 * p.q_head;
+  uint32_t qa[KS][4];
+#pragma unroll
+  for (int k = 0; k < KS; ++k)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int r = ra + (e & 1) * 8, c = k * 16 + (e >> 1) * 8 + (lane & 3) * 2;
+      qa[k][e] = r < nh ? *reinterpret_cast<const uint32_t*>(q + r * p.q_head + c) : 0u;
+    }
+  float o[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  Running run;
+  for (int u = u0; u < u1; ++u) {
+    if (u + 1 < u1) {
+      load(u + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncwarp();
+    if (ok_bits >> (u & 1) & 1) {
+      const uint8_t* sk = ring + (u & 1) * 2 * TILE;
+      float sc[2][4] = {};
+      scores<T, D>(sk, 0, qa, sc);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = begin + u * kUnit + t * 8 + (lane & 3) * 2 + (e & 1);
+          sc[t][e] = key < len ? sc[t][e] * p.scale_log2 : -INFINITY;
+        }
+      float fa, fb;
+      uint32_t pa[4];
+      softmax_step<T>(sc, run, fa, fb, pa);
+      add_values<T, D>(sk + TILE, 0, pa, fa, fb, o);
+    }
+    __syncwarp();  // the stage may be loaded again
+  }
+  join_lanes(run);
+
+  const int splits = p.prefix_splits + p.own_splits;
+  if (p.own_splits > 1) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int r = ra + half * 8;
+      if (r >= nh) continue;
+      const long long slot = ((long long)b * p.heads + h0 + r) * splits + p.prefix_splits + split;
+      const float mm = half ? run.mb : run.ma, ll = half ? run.lb : run.la;
+      if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm, ll);
+      if (mm == -INFINITY && ll == 0.f) continue;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        *reinterpret_cast<float2*>(p.part_o + slot * D + t * 8 + (lane & 3) * 2) =
+            make_float2(o[t][2 * half], o[t][2 * half + 1]);
+    }
+    return;
+  }
+  // the prefix ranges of these heads join here
+  unsigned bad = 0;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = ra + half * 8;
+    const bool mine = r < nh;
+    const long long slot = ((long long)b * p.heads + h0 + (mine ? r : 0)) * splits;
+    float m = half ? run.mb : run.ma, l = half ? run.lb : run.la;
+    if (group >= 0 && mine) {
+      for (int i = 0; i < p.prefix_splits; ++i) {
+        const float2 ml = p.part_ml[slot + i];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float n = fmaxf(m, ml.x), sh = softmax_shift(n);
+        const float fo = ex2_approx(m - sh), fp = ex2_approx(ml.x - sh);
+        l = l * fo + ml.y * fp;
+        m = n;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float2 y = *reinterpret_cast<const float2*>(p.part_o + (slot + i) * D + t * 8 + (lane & 3) * 2);
+          o[t][2 * half] = o[t][2 * half] * fo + y.x * fp;
+          o[t][2 * half + 1] = o[t][2 * half + 1] * fo + y.y * fp;
+        }
+      }
+    }
+    const float inv = len > 0 ? 1.f / l : 0.f;  // an empty sequence gives zeros
+    bool ok = len == 0 || (l > 0.f && finite_f(l));
+    T* out = static_cast<T*>(p.out) + b * p.o_row + (h0 + r) * p.o_head;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      ok = ok && finite_f(o[t][2 * half]) && finite_f(o[t][2 * half + 1]);
+      if (mine)
+        *reinterpret_cast<uint32_t*>(out + t * 8 + (lane & 3) * 2) =
+            Elem<T>::pack(o[t][2 * half] * inv, o[t][2 * half + 1] * inv);
+    }
+    const unsigned votes = __ballot_sync(0xffffffffu, mine && !ok);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (votes >> (4 * i) & 0xf) bad |= 1u << (half * 8 + i);
+  }
+  __syncwarp();
+  for (int r = 0; bad >> r; ++r)
+    if (bad >> r & 1) row_again<T, D>(p, b, h0 + r);
+}
+
+// Joins the ranges of each (row, head): a warp each, D / 32 dims per lane.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
+  constexpr int DV = D / 32;
+  pdl_trigger();
+  pdl_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long item = (long long)blockIdx.x * (kThreads / 32) + warp;
+  if (item >= (long long)p.rows * p.heads) return;
+  const int b = (int)(item / p.heads), h = (int)(item - (long long)b * p.heads);
+  const int splits = p.prefix_splits + p.own_splits;
+  const int first = p.prefix_splits && row_group(p, b) >= 0 ? 0 : p.prefix_splits;
+  int s;
+  const int len = row_length(p, b, &s);
+  float m = -INFINITY, l = 0.f, o[DV] = {};
+  for (int i = first; i < splits; ++i) {
+    const float2 ml = p.part_ml[item * splits + i];
+    if (ml.x == -INFINITY && ml.y == 0.f) continue;
+    const float n = fmaxf(m, ml.x), sh = softmax_shift(n);
+    const float fo = ex2_approx(m - sh), fp = ex2_approx(ml.x - sh);
+    l = l * fo + ml.y * fp;
+    m = n;
+    const float* y = p.part_o + (item * splits + i) * D + lane * DV;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = o[d] * fo + y[d] * fp;
+  }
+  bool ok = len == 0 || (l > 0.f && finite_f(l));
+#pragma unroll
+  for (int d = 0; d < DV; ++d) ok = ok && finite_f(o[d]);
+  if (__any_sync(0xffffffffu, !ok)) {
+    row_again<T, D>(p, b, h);
+    return;
+  }
+  const float inv = len > 0 ? 1.f / l : 0.f;
+  T* out = static_cast<T*>(p.out) + b * p.o_row + h * p.o_head + lane * DV;
+#pragma unroll
+  for (int d = 0; d < DV; d += 2) *reinterpret_cast<uint32_t*>(out + d) = Elem<T>::pack(o[d] * inv, o[d + 1] * inv);
+}
+
+// Splits and tiles of a call, from the shapes and the caller's hints alone.
+void plan(const OasisSharedArgs* a, SharedParams* p) {
+  const int sms = num_sms();
+  const int K = a->cache->kv_heads;
+  p->per = a->heads / K;
+  p->head_tiles = (p->per + 15) / 16;
+  const bool prefix = a->groups > 0 && a->prefix_pages_hint > 0;
+  const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
+  p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);
+  p->prefix_splits = 0;
+  if (prefix) {
+    // two blocks for each SM, and at least 128 keys for each block
+    const long long blocks = (long long)a->groups * K * p->tiles;
+    const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
+    long long n = (2LL * sms + blocks - 1) / blocks;
+    if (n > keys / 128) n = keys / 128;
+    p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+  }
+  // eight warps for each SM, and at least 64 keys for each warp
+  const long long items = (long long)a->rows * K * p->head_tiles;
+  const long long own = a->own_tokens_hint;
+  long long n = (8LL * sms + items - 1) / items;
+  if (n > own / 64) n = own / 64;
+  p->own_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+}
+
+size_t partial_bytes(const OasisSharedArgs* a, const SharedParams& p) {
+  if (p.prefix_splits == 0 && p.own_splits == 1) return 0;
+  const size_t slots = (size_t)a->rows * a->heads * (p.prefix_splits + p.own_splits);
+  return slots * (sizeof(float2) + sizeof(float) * a->cache->head_dim);
+}
+
+template <typename T, int D>
+int launch(const SharedParams& p, cudaStream_t s) {
+  static std::atomic<bool> attr[64];  // per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    cudaError_t e =
+        cudaFuncSetAttribute(shared_prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<D>());
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(shared_own_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem<D>());
+    if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    attr[dev & 63] = true;
+  }
+  if (p.prefix_splits) {
+    const long long blocks = (long long)p.groups * p.g.kv_heads * p.prefix_splits * p.tiles;
+    launch_pdl(shared_prefix_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
+    OASIS_TRY(check_launch("shared_prefix_kernel"));
+  }
+  const long long items = (long long)p.rows * p.g.kv_heads * p.head_tiles * p.own_splits;
+  launch_pdl(shared_own_kernel<T, D>, dim3((unsigned)((items + kOwnWarps - 1) / kOwnWarps)), dim3(kOwnWarps * 32),
+             own_smem<D>(), s, p);
+  OASIS_TRY(check_launch("shared_own_kernel"));
+  if (p.own_splits > 1) {
+    const long long rows = (long long)p.rows * p.heads;
+    launch_pdl(shared_join_kernel<T, D>, dim3((unsigned)((rows + kThreads / 32 - 1) / (kThreads / 32))), dim3(kThreads),
+               0, s, p);
+    OASIS_TRY(check_launch("shared_join_kernel"));
+  }
+  return OASIS_OK;
+}
+
+int check_shared(const OasisSharedArgs* a) {
+  OASIS_REQUIRE(a && a->cache, "attention_shared: null args");
+  const OasisPageCache* c = a->cache;
+  OASIS_REQUIRE(c->dtype == OASIS_DTYPE_BF16 || c->dtype == OASIS_DTYPE_F16, "attention_shared: dtype=%d", c->dtype);
+  OASIS_REQUIRE(c->head_dim == 64 || c->head_dim == 128, "attention_shared: head_dim=%d is not 64 or 128", c->head_dim);
+  OASIS_REQUIRE(c->pages >= 1 && c->layers >= 1 && c->kv_heads >= 1 && c->slots >= 1 && c->width >= 1,
+                "attention_shared: pages=%d layers=%d kv_heads=%d slots=%d width=%d", c->pages, c->layers, c->kv_heads,
+                c->slots, c->width);
+  OASIS_REQUIRE(c->page_size >= 16 && c->page_size <= 256 && c->page_size % 16 == 0,
+                "attention_shared: page_size=%d is not a multiple of 16 up to 256", c->page_size);
+  OASIS_REQUIRE((long long)c->slots * c->width < (1LL << 31) && (long long)c->width * c->page_size < (1LL << 31),
+                "attention_shared: page table of %d x %d entries is too large", c->slots, c->width);
+  OASIS_REQUIRE(a->layer >= 0 && a->layer < c->layers, "attention_shared: layer=%d of %d", a->layer, c->layers);
+  OASIS_REQUIRE(a->heads >= c->kv_heads && a->heads <= 1024 && a->heads % c->kv_heads == 0,
+                "attention_shared: heads=%d kv_heads=%d", a->heads, c->kv_heads);
+  OASIS_REQUIRE(a->rows >= 0 && a->groups >= 0, "attention_shared: rows=%d groups=%d", a->rows, a->groups);
+  OASIS_REQUIRE(a->scale > 0.f && a->scale <= 3e38f, "attention_shared: scale=%g", (double)a->scale);
+  return OASIS_OK;
+}
+
+}  // namespace
+}  // namespace oasis
+
+using namespace oasis;
+
+extern "C" {
+
+size_t oasis_attention_shared_workspace_size(const OasisSharedArgs* a) {
+  if (check_shared(a) != OASIS_OK || a->rows == 0) return 0;
+  SharedParams p;
+  plan(a, &p);
+  return partial_bytes(a, p);
+}
+
+int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream) {
+  OASIS_TRY(check_shared(a));
+  if (a->rows == 0) return OASIS_OK;
+  const OasisPageCache* c = a->cache;
+  OASIS_REQUIRE(a->q && a->out && a->seqs && c->pool && c->table && c->lengths && c->status,
+                "attention_shared: null pointer");
+  OASIS_REQUIRE(a->groups == 0 || (a->group_start && a->prefix_pages), "attention_shared: null group arrays");
+  const uintptr_t at = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out) |
+                       reinterpret_cast<uintptr_t>(c->pool);
+  OASIS_REQUIRE((at & 15) == 0, "attention_shared: operands not 16-byte aligned");
+  const long long strides[4] = {a->q_row_stride, a->q_head_stride, a->out_row_stride, a->out_head_stride};
+  for (long long s : strides)
+    OASIS_REQUIRE(s > 0 && s % 8 == 0 && s < (1LL << 36),
+                  "attention_shared: stride %lld is not a positive multiple of 8 elements", s);
+  SharedParams p;
+  plan(a, &p);
+  const long long blocks = (long long)a->groups * c->kv_heads * (p.prefix_splits ? p.prefix_splits : 1) * p.tiles;
+  const long long items = (long long)a->rows * c->kv_heads * p.head_tiles * p.own_splits;
+  OASIS_REQUIRE(blocks < (1LL << 31) && items < (1LL << 31), "attention_shared: %d rows of %d heads are too many",
+                a->rows, a->heads);
+  const size_t want = partial_bytes(a, p);
+  if (want && (!a->workspace || a->workspace_bytes < want))
+    return set_error(OASIS_ERR_WORKSPACE, "attention_shared: workspace of %zu bytes, %zu needed", a->workspace_bytes,
+                     want);
+  OASIS_REQUIRE((reinterpret_cast<uintptr_t>(a->workspace) & 15) == 0, "attention_shared: workspace not 16-byte aligned");
+  p.g.pages = c->pages;
+  p.g.layers = c->layers;
+  p.g.kv_heads = c->kv_heads;
+  p.g.page_size = c->page_size;
+  p.g.head_dim = c->head_dim;
+  p.g.slots = c->slots;
+  p.g.width = c->width;
+  p.q = a->q;
+  p.out = a->out;
+  p.pool = c->pool;
+  p.q_row = strides[0];
+  p.q_head = strides[1];
+  p.o_row = strides[2];
+  p.o_head = strides[3];
+  p.table = c->table;
+  p.lengths = c->lengths;
+  p.seqs = a->seqs;
+  p.group_start = a->group_start;
+  p.prefix_pages = a->prefix_pages;
+  p.status = c->status;
+  p.part_o = static_cast<float*>(a->workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a->rows * a->heads * (p.prefix_splits + p.own_splits) *
+                                                       c->head_dim);
+  p.rows = a->rows;
+  p.groups = a->groups;
+  p.heads = a->heads;
+  p.layer = a->layer;
+  p.scale_log2 = a->scale * kLog2e;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (c->dtype == OASIS_DTYPE_BF16)
+    return c->head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+  return c->head_dim == 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
+}
+
+}  // extern "C"

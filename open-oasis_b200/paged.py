@@ -203,3 +203,61 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
                              k.shape[1], dim, DTYPES[q.dtype], dim ** -0.5 if scale is None else scale)
     _lib.call("oasis_attention_prompt", C.byref(a), _stream(stream))
     return out
+
+
+class SharedPlan:
+    """Which rows of a batch share a prefix: group g is the next group_rows[g] rows, and
+    the first prefix_pages[g] pages of their sequences are the same (PagedCache.fork
+    leaves them so). `longest`: the most tokens of a sequence in the calls to come (a
+    hint that chooses splits). Made once for a batch and kept while it lasts."""
+
+    def __init__(self, group_rows: list[int], prefix_pages: list[int], longest: int, device="cuda"):
+        if len(group_rows) != len(prefix_pages) or any(r < 0 for r in group_rows) or any(p < 0 for p in prefix_pages):
+            raise ValueError("group_rows and prefix_pages must hold one count, not negative, for each group")
+        starts = [0]
+        for r in group_rows:
+            starts.append(starts[-1] + r)
+        self.groups, self.rows = len(group_rows), starts[-1]
+        self.group_start = torch.tensor(starts, dtype=torch.int32, device=device)
+        self.prefix_pages = torch.tensor(prefix_pages or [0], dtype=torch.int32, device=device)
+        self.longest = longest
+        self.most_rows = max(group_rows, default=0)
+        self.most_pages = max(prefix_pages, default=0)
+        self.least_pages = min(prefix_pages, default=0)
+
+
+def attention_shared(q: torch.Tensor, cache: PagedCache, layer: int, seqs: torch.Tensor, plan: SharedPlan,
+                     out: torch.Tensor | None = None, scale: float | None = None, stream=None) -> torch.Tensor:
+    """One query per row: q [rows, heads, head_dim] over the tokens of sequences
+    seqs [rows] of the cache, in one layer, after their newest token was written.
+    Prefixes that `plan` names are read once for their group."""
+    device = q.device
+    _check_device(device)
+    if cache.device != device or plan.group_start.device != device:
+        raise ValueError(f"q is on {device}, the cache on {cache.device}, the plan on {plan.group_start.device}")
+    _check_rows(q, "q", cache.dtype, device, None, cache.head_dim)
+    rows, heads, dim = q.shape
+    _check_ints(seqs, "seqs", device, rows)
+    if plan.rows > rows:
+        raise ValueError(f"the plan is for {plan.rows} rows, q has {rows}")
+    if out is None:
+        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=device)
+        if stream is not None:
+            out.record_stream(stream)
+    else:
+        _check_rows(out, "out", q.dtype, device, heads, dim)
+        if out.shape[0] != rows:
+            raise ValueError(f"out has {out.shape[0]} rows, q {rows}")
+    own = max(0, plan.longest - plan.least_pages * cache.page_size)
+    a = _lib.OasisSharedArgs(q.data_ptr(), out.data_ptr(), *_strides(q), *_strides(out), C.pointer(cache._c), layer,
+                             seqs.data_ptr(), rows, heads, plan.group_start.data_ptr(), plan.prefix_pages.data_ptr(),
+                             plan.groups, plan.most_rows, plan.most_pages, own, dim ** -0.5 if scale is None else scale)
+    ref = C.byref(a)
+    size = _lib.load().oasis_attention_shared_workspace_size(ref)
+    if size:
+        ws = workspace(size, device)
+        if stream is not None:
+            ws.record_stream(stream)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), size
+    _lib.call("oasis_attention_shared", ref, _stream(stream))
+    return out

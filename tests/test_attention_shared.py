@@ -1,0 +1,393 @@
+"""Attention of single queries over the paged cache, with and without shared prefixes,
+against fp64 within the bound of its roundings; then the operators in a run."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+import os
+import random
+import subprocess
+import tempfile
+
+import pytest
+import torch
+
+from oasis_b200 import _lib, paged
+from oracle import paged_oracle as O
+from tests.helpers import ROOT
+
+DEV = "cuda"
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def ints(v):
+    return torch.tensor(v, dtype=torch.int32, device=DEV)
+
+
+def build(groups, page, heads_kv, dim, dtype, seed=0, layers=2):
+    """A cache with a scattered table. groups: (prefix pages, [length of each row])."""
+    rng = random.Random(seed)
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    lists, lengths = [], []
+    need = sum(p + sum(-(-max(0, t - p * page) // page) for t in ls) for p, ls in groups)
+    order = list(range(need + 3))
+    rng.shuffle(order)
+    take = lambda n: [order.pop() for _ in range(n)]  # noqa: E731
+    for p, ls in groups:
+        common = take(p)
+        for t in ls:
+            lists.append((common + take(-(-max(0, t - p * page) // page)))[: -(-t // page)])
+            lengths.append(t)
+    n = len(lists)
+    slots = list(range(n + 2))
+    rng.shuffle(slots)
+    seqs = slots[:n]
+    width = max(1, max(len(x) for x in lists))
+    c = paged.PagedCache(need + 3, page, layers, heads_kv, dim, n + 2, width, dtype=dtype, device=DEV)
+    c.pool.normal_(generator=g)
+    for s, pages, t in zip(seqs, lists, lengths):
+        c.table[s, : len(pages)] = ints(pages)
+        c.lengths[s] = t
+    plan = paged.SharedPlan([len(ls) for _, ls in groups], [p for p, _ in groups], max(lengths), DEV)
+    return c, seqs, plan, g
+
+
+def queries(n, heads, dim, dtype, gen, scale=2.0):
+    return torch.empty(n, heads, dim, dtype=dtype, device=DEV).normal_(generator=gen).mul_(scale)
+
+
+def check(got, q, c, layer, seqs, scale=None, rows=None):
+    table, lengths = c.table.tolist(), c.lengths.tolist()
+    want = O.attention_cached(q, c.pool, table, lengths, layer, seqs, scale)
+    absolute = c.pool.clone()
+    absolute[:, :, 1] = absolute[:, :, 1].abs()
+    spread = O.attention_cached(q, absolute, table, lengths, layer, seqs, scale)
+    scale_ = q.shape[2] ** -0.5 if scale is None else scale
+    finite = torch.nan_to_num(c.pool[:, layer, 0].double(), 0, 0, 0)
+    finite = torch.where(finite.abs() > 1e30, 0, finite)  # such a key's probability is 0
+    reach = scale_ * float(torch.nan_to_num(q.double()).norm(dim=-1).max() * finite.norm(dim=-1).max())
+    bound = O.error_bound(want, spread, reach, max(lengths), q.shape[2], q.dtype)
+    off = (got.double() - want).abs()
+    rows = slice(None) if rows is None else rows
+    assert bool((off <= bound)[rows].all()), float((off / bound)[rows].max())
+    return want
+
+
+# ----------------------------------------------------------------- without a GPU --
+
+def _args(cache=None, **kw):
+    c = dict(pool=16, pages=4, layers=1, kv_heads=1, page_size=16, head_dim=64, dtype=1, table=16, slots=2, width=2,
+             lengths=16, refs=16, status=16)
+    c.update(cache or {})
+    keep = _lib.OasisPageCache(**c)
+    a = dict(q=16, out=16, q_row_stride=64, q_head_stride=64, out_row_stride=64, out_head_stride=64,
+             cache=C.pointer(keep), layer=0, seqs=16, rows=1, heads=1, scale=0.125)
+    a.update(kw)
+    return _lib.OasisSharedArgs(**a), keep
+
+
+@pytest.mark.parametrize("cache,kw,text", [
+    (dict(dtype=0), {}, b"dtype"), (dict(head_dim=96), {}, b"head_dim=96"), (dict(page_size=8), {}, b"page_size=8"),
+    (dict(width=1 << 30), {}, b"too large"), (dict(pool=0), {}, b"null"), (dict(pool=8), {}, b"16-byte"),
+    ({}, dict(layer=1), b"layer=1"), ({}, dict(layer=-1), b"layer=-1"), (dict(kv_heads=2), dict(heads=3), b"heads=3"),
+    ({}, dict(rows=-1), b"rows=-1"), ({}, dict(groups=-1), b"groups=-1"), ({}, dict(scale=0.0), b"scale"),
+    ({}, dict(scale=math.nan), b"scale"), ({}, dict(q=0), b"null"), ({}, dict(out=24), b"16-byte"),
+    ({}, dict(q_row_stride=4), b"stride"), ({}, dict(groups=1), b"group arrays"),
+    (dict(kv_heads=4), dict(rows=1 << 30, heads=4), b"too many"),
+])
+def test_arguments_are_checked(cache, kw, text):
+    a, _ = _args(cache, **kw)
+    lib = _lib.load()
+    assert lib.oasis_attention_shared(C.byref(a), None) == -1
+    assert text in lib.oasis_last_error()
+
+
+def test_workspace_is_asked_for():
+    lib = _lib.load()
+    a, _ = _args(rows=2, groups=1, group_start=16, prefix_pages=16, group_rows_hint=2, prefix_pages_hint=40)
+    size = lib.oasis_attention_shared_workspace_size(C.byref(a))
+    assert size > 0
+    for ws, n in ((0, size), (16, size - 1)):
+        a.workspace, a.workspace_bytes = ws, n
+        assert lib.oasis_attention_shared(C.byref(a), None) == -3 and b"workspace" in lib.oasis_last_error()
+    a, _ = _args(rows=0)
+    assert lib.oasis_attention_shared_workspace_size(C.byref(a)) == 0
+    assert lib.oasis_attention_shared(C.byref(a), None) == 0
+    assert lib.oasis_attention_shared(None, None) == -1
+
+
+def test_struct_layout_matches_c():
+    with tempfile.TemporaryDirectory() as d:
+        lines = [f'printf("%zu\\n", offsetof(OasisSharedArgs, {f}));' for f, _ in _lib.OasisSharedArgs._fields_]
+        f, exe = os.path.join(d, "l.c"), os.path.join(d, "l")
+        open(f, "w").write('#include <stdio.h>\n#include <stddef.h>\n' + f'#include "{ROOT}/include/oasis_b200.h"\n'
+                           + "int main(void) {" + "".join(lines) + 'printf("%zu\\n", sizeof(OasisSharedArgs)); return 0; }')
+        subprocess.run(["gcc", "-std=c99", f, "-o", exe], check=True)
+        got = [int(x) for x in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split()]
+    want = [getattr(_lib.OasisSharedArgs, f).offset for f, _ in _lib.OasisSharedArgs._fields_]
+    assert got == want + [C.sizeof(_lib.OasisSharedArgs)]
+
+
+def test_plan_is_checked():
+    with pytest.raises(ValueError, match="group_rows"):
+        paged.SharedPlan([1, 2], [3], 10, "cpu")
+    with pytest.raises(ValueError, match="group_rows"):
+        paged.SharedPlan([1, -2], [3, 0], 10, "cpu")
+
+
+# --------------------------------------------------------------------- on a GPU --
+
+GROUPS = {
+    "one row": [(0, [1])],
+    "lengths": [(0, [1, 15, 16, 17, 0, 64, 65, 200])],
+    "prefix": [(2, [33, 40, 32, 64])],
+    "no own": [(3, [48, 48])],
+    "several": [(1, [20, 17]), (0, [5, 0, 31]), (9, [145, 300, 151]), (2, [32])],
+    "shorter than the prefix": [(4, [10, 64, 0, 50, 90])],
+    "all short": [(4, [10, 0, 20])],
+    "many rows": [(5, [80 + i % 7 for i in range(70)])],
+    "long": [(60, [1000, 1900, 961]), (0, [1500, 3])],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", GROUPS)
+@pytest.mark.parametrize("heads,kv,dim,dtype,page", [
+    (2, 2, 64, BF16, 16), (6, 2, 128, BF16, 16), (4, 1, 64, FP16, 32), (7, 1, 128, FP16, 48), (40, 2, 64, BF16, 64),
+])
+def test_groups(name, heads, kv, dim, dtype, page):
+    groups = [(-(-p * 16 // page), [t if t < p * 16 else t + (-(-p * 16 // page)) * page - p * 16 for t in ls])
+              for p, ls in GROUPS[name]]
+    c, seqs, plan, g = build(groups, page, kv, dim, dtype)
+    q = queries(len(seqs), heads, dim, dtype, g)
+    got = paged.attention_shared(q, c, 1, ints(seqs), plan)
+    check(got, q, c, 1, seqs)
+    alone = paged.SharedPlan([], [], plan.longest, DEV)
+    check(paged.attention_shared(q, c, 1, ints(seqs), alone), q, c, 1, seqs)
+    c.check()
+
+
+@pytest.mark.gpu
+def test_hints_only_choose_the_split():
+    c, seqs, plan, g = build([(30, [500, 900, 700]), (0, [1200])], 16, 2, 64, BF16)
+    q = queries(4, 4, 64, BF16, g)
+    for longest, rows, pages in ((1, 1, 1), (1 << 20, 1000, 1), (900, 1, 4000), (10, 3, 0)):
+        plan.longest, plan.most_rows, plan.most_pages, plan.least_pages = longest, rows, pages, 0
+        check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+
+
+@pytest.mark.gpu
+def test_rows_outside_the_groups_and_named_twice():
+    c, seqs, _, g = build([(2, [40, 50, 33])], 16, 1, 64, BF16)
+    plan = paged.SharedPlan([2], [2], 64, DEV)
+    plan.group_start += 1  # rows 1 and 2
+    order = [seqs[2], seqs[0], seqs[1], seqs[0], seqs[2]]
+    q = queries(5, 2, 64, BF16, g)
+    check(paged.attention_shared(q, c, 0, ints(order), plan), q, c, 0, order)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_what_lies_behind_a_sequence_takes_no_part(dim, bad):
+    """NaN in pages behind a sequence's last token, and in the prefix behind a shorter
+    row; NaN and empty results where the formula has them."""
+    groups = [(3, [20, 70, 52, 0, 48]), (0, [7])]
+    c, seqs, plan, g = build(groups, 16, 2, dim, BF16)
+    lists, lengths = c.table.tolist(), c.lengths.tolist()
+    for s in seqs:
+        t = lengths[s]
+        if t % 16 and t >= 48 or t == 7:
+            c.pool[lists[s][t // 16], :, :, :, t % 16:] = bad
+    unused = [p for p in range(c.pages) if all(p not in r for r in lists)]
+    c.pool[unused] = bad
+    q = queries(6, 6, dim, BF16, g)
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    check(got, q, c, 0, seqs)
+    c.pool[lists[seqs[1]][2], :, :, :, 5] = bad  # token 37 of the prefix: rows 1, 2 and 4 see it, row 0 does not
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    want = check(got, q, c, 0, seqs, rows=[0, 3, 5])
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and bool(torch.isnan(want[[1, 2, 4]]).any())
+    q[1] = math.nan
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    check(got, q, c, 0, seqs, rows=[0, 3, 5])
+    assert bool(torch.isnan(got[1]).all())
+
+
+@pytest.mark.gpu
+def test_lowest_scores():
+    """Keys that score -inf or the lowest value: in the whole prefix, in a row's own part."""
+    c, seqs, plan, g = build([(4, [70, 100])], 16, 1, 64, BF16)
+    q = queries(2, 2, 64, BF16, g)
+    q[:, :, 0] = 1
+    c.pool[..., 0] = torch.where(torch.arange(2, device=DEV)[None, None, :, None, None] == 0, 0, c.pool[..., 0])
+    common = c.table[seqs[0], :4].long()
+    c.pool[common, :, 0, :, :, 0] = -math.inf
+    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    c.pool[common, :, 0, :, :, 0] = torch.finfo(BF16).min
+    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    c.pool[:, :, 0, :, :, 0] = -math.inf
+    assert bool(torch.isnan(paged.attention_shared(q, c, 0, ints(seqs), plan)).all())  # as the formula: 0 / 0
+
+
+@pytest.mark.gpu
+def test_bad_indexes_are_left_out():
+    c, seqs, plan, g = build([(2, [40, 40]), (0, [64, 20])], 16, 1, 64, BF16)
+    q = queries(4, 1, 64, BF16, g)
+    good = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    table = c.table.clone()
+    c.table[seqs[2], 1] = 1 << 30
+    c.table[seqs[3], :2] = ints([-1, c.pages])
+    got = paged.attention_shared(q, c, 0, ints([seqs[0], 99, seqs[2], seqs[3]]), plan)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], good[0]) and not bool(got[1].any()) and not bool(got[3].any())
+    assert int(c.status.item()) == paged.BAD_SEQUENCE | paged.BAD_PAGE
+    c.table.copy_(table)
+    pages = c.table[seqs[2], :4].tolist()
+    short = O.attention_rows(q[2:3], c.pool[[pages[0], pages[2], pages[3]], 0, 0].transpose(1, 2).reshape(-1, 1, 64),
+                             c.pool[[pages[0], pages[2], pages[3]], 0, 1].transpose(1, 2).reshape(-1, 1, 64))
+    assert float((got[2].double() - short[0]).norm() / short.norm()) < 2 * 2.0 ** -8
+
+
+@pytest.mark.gpu
+def test_strides_streams_graph():
+    c, seqs, plan, g = build([(20, [330, 400]), (0, [100])], 16, 2, 64, BF16)
+    rows = torch.empty(3, 8, 64, dtype=BF16, device=DEV).normal_(generator=g)
+    q = rows[:, 2:6]  # a view of packed rows
+    out = torch.zeros(4, 3, 2, 64, dtype=BF16, device=DEV)[:, :, 0].transpose(0, 1)  # heads outside
+    at = ints(seqs)
+    paged.attention_shared(q, c, 1, at, plan, out=out)
+    check(out, q, c, 1, seqs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    a = paged.attention_shared(q, c, 1, at, plan, stream=side)
+    b = paged.attention_shared(q, c, 1, at, plan)  # beside it, each with its own workspace
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(a, b) and torch.equal(a, out)
+    graphs, outs = [], []
+    for _ in range(2):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            outs.append(paged.attention_shared(q, c, 1, at, plan))
+        graphs.append(gr)
+    side.wait_stream(torch.cuda.current_stream())
+    for gr in graphs:
+        gr.replay()
+    with torch.cuda.stream(side):
+        graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], a) and torch.equal(outs[1], a)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """A pool of more than 2^32 bytes: pages at its far end."""
+    c = paged.PagedCache(4100, 64, 8, 8, 128, 2, 3, device=DEV)  # 8.6 GB
+    assert c.pool.numel() > 1 << 32
+    pages = [4099, 0, 4098]
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for p in pages:
+        c.pool[p].normal_(generator=g)
+    c.table[1] = ints(pages)
+    c.lengths[1] = 150
+    c.refs[pages] = 1
+    q = queries(1, 8, 128, BF16, g)
+    small = paged.PagedCache(3, 64, 8, 8, 128, 2, 3, device=DEV)
+    small.pool.copy_(c.pool[pages])
+    small.table[1] = ints([0, 1, 2])
+    small.lengths[1] = 150
+    plan = paged.SharedPlan([1], [2], 192, DEV)
+    a = paged.attention_shared(q, c, 7, ints([1]), plan)
+    b = paged.attention_shared(q, small, 7, ints([1]), plan)
+    assert torch.equal(a, b)
+    check(b, q, small, 7, [1])
+    rows = torch.empty(10, 8, 128, dtype=BF16, device=DEV).normal_(generator=g)
+    for x in (c, small):
+        start = x.reserve(ints([1]), ints([0, 10]))
+        x.write(7, rows, rows, ints([1]), ints([0, 10]), start)
+    assert torch.equal(c.pool[4098], small.pool[2])
+    c.compact()  # the far pages move to 1 and 2
+    assert c.table[1].tolist() == [1 if p == 4098 else 2 if p == 4099 else 0 for p in pages]
+    assert torch.equal(c.pool[c.table[1].long()], small.pool)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16)])
+def test_a_run_of_them_together(dim, dtype):
+    """Two prompts enter, are forked, grow token by token, one branch ends, the pool is
+    compacted and the rest goes on: each step's attention against fp64 over the
+    tokens that each sequence really holds."""
+    rng = random.Random(3)
+    heads, kv, page, layers = 6, 2, 16, 2
+    c = paged.PagedCache(40, page, layers, kv, dim, 8, 10, dtype=dtype, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(4)
+    held = {}  # sequence -> per layer list of (k, v) rows
+
+    def rows(n):
+        return torch.empty(layers, n, heads + 2 * kv, dim, dtype=dtype, device=DEV).normal_(generator=g)
+
+    lengths = [70, 37]
+    x = rows(sum(lengths))
+    cu = [0, 70, 107]
+    start = c.reserve(ints([0, 1]), ints(cu))
+    for layer in range(layers):
+        q, k, v = x[layer, :, :heads], x[layer, :, heads : heads + kv], x[layer, :, heads + kv :]
+        got = paged.attention_prompt(q, k, v, ints(cu), 70)
+        want, spread = O.attention_prompt(q, k, v, cu), O.attention_prompt(q, k, v.abs(), cu)
+        reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max())
+        assert bool(((got.double() - want).abs() <= O.error_bound(want, spread, reach, 70, dim, dtype)).all())
+        c.write(layer, k, v, ints([0, 1]), ints(cu), start)
+    for i, s in enumerate((0, 1)):
+        held[s] = x[:, cu[i] : cu[i + 1], heads:].clone()
+    c.fork(ints([0, 0, 1]), ints([2, 3, 4]))
+    for s, t in ((0, 2), (0, 3), (1, 4)):
+        held[t] = held[s].clone()
+    order, plan = [0, 2, 3, 1, 4], paged.SharedPlan([3, 2], [70 // page, 37 // page], 100, DEV)
+    for step in range(24):
+        if step == 9:  # a branch ends
+            c.free(ints([2]))
+            del held[2]
+            order, plan = [0, 3, 1, 4], paged.SharedPlan([2, 2], [70 // page, 37 // page], 100, DEV)
+            c.compact()
+        if step == 15:  # and its slot takes a copy of another
+            c.fork(ints([3]), ints([2]), deep=True)
+            held[2] = held[3].clone()
+            order, plan = [0, 3, 1, 4, 2], paged.SharedPlan([2, 2], [70 // page, 37 // page], 100, DEV)
+        n = len(order)
+        x = rows(n)
+        one = list(range(n + 1))
+        start = c.reserve(ints(order), ints(one))
+        for layer in range(layers):
+            c.write(layer, x[layer, :, heads : heads + kv], x[layer, :, heads + kv :], ints(order), ints(one), start)
+            got = paged.attention_shared(x[layer, :, :heads], c, layer, ints(order), plan)
+            for i, s in enumerate(order):
+                if layer == 0:
+                    held[s] = torch.cat([held[s], x[:, i : i + 1, heads:]], 1)
+                k, v = held[s][layer, :, :kv], held[s][layer, :, kv:]
+                q = x[layer, i : i + 1, :heads]
+                want, spread = O.attention_rows(q, k, v), O.attention_rows(q, k, v.abs())
+                reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max())
+                bound = O.error_bound(want, spread, reach, k.shape[0], dim, dtype)
+                assert bool(((got[i : i + 1].double() - want).abs() <= bound).all()), (step, layer, s)
+    c.check()
+    assert sorted(c.lengths.tolist()) == sorted(held[s].shape[1] if s in held else 0 for s in range(8))
+    c.free(ints(list(range(8))))
+    assert not bool(c.refs.any()) and rng
+
+
+@pytest.mark.gpu
+def test_python_checks():
+    c, seqs, plan, g = build([(1, [20, 20])], 16, 1, 64, BF16)
+    q = queries(2, 1, 64, BF16, g)
+    at = ints(seqs)
+    call = paged.attention_shared
+    for args, text in (((q.half(), c, 0, at, plan), "q must be"), ((q[:1], c, 0, at, plan), "seqs must hold 1"),
+                       ((q, c, 0, at.long(), plan), "int32"), ((q[:1], c, 0, at[:1], plan), "plan is for 2"),
+                       ((q.cpu(), c, 0, at, plan), "CUDA")):
+        with pytest.raises(ValueError, match=text):
+            call(*args)
+    with pytest.raises(ValueError, match="out has 3"):
+        call(q, c, 0, at, plan, out=torch.zeros(3, 1, 64, dtype=BF16, device=DEV))
+    with pytest.raises(_lib.OasisError, match="layer=2"):
+        call(q, c, 2, at, plan)
+    assert call(q[:0], c, 0, at[:0], paged.SharedPlan([], [], 1, DEV)).shape == (0, 1, 64)
