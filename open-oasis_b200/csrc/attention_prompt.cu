@@ -23,6 +23,9 @@ namespace {
 constexpr int kRowsTile = 64;  // query rows of a block, and keys of a step
 constexpr int kRowsThreads = 128;
 
+// Up to this length the rows kernel is taken.
+constexpr int kShort = 64;
+
 template <int D>
 constexpr int rows_smem() {
   return 5 * kRowsTile * D * 2;  // Q (then O), two K and two V tiles
@@ -283,5 +286,6 @@ extern "C" int oasis_attention_prompt(const OasisPromptArgs* a, oasis_stream_t s
   p.head_dim = a->head_dim;
   p.dtype = a->dtype;
   p.scale_log2 = a->scale * kLog2e;
-  return prompt_rows_launch(p, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a->longest <= kShort ? prompt_rows_launch(p, st) : prompt_tc_launch(p, st);
 }

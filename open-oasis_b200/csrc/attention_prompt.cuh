@@ -15,5 +15,7 @@ struct PromptParams {
 };
 
 int prompt_rows_launch(const PromptParams& p, cudaStream_t s);
+int prompt_tc_launch(const PromptParams& p, cudaStream_t s);
+int read_device_error_prompt(int reset);
 
 }  // namespace oasis

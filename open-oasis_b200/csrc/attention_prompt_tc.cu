@@ -1,0 +1,506 @@
+// Causal attention over packed prompts on the 5th-generation tensor cores: the kernel
+// for sequences that are not short (attention_prompt.cu has the formula and the
+// kernel for short ones).
+//
+// A block takes two tiles of 128 query rows that read the same keys: the same rows of
+// two heads of one key head where heads come in even groups (both tiles then see the
+// same key range), otherwise 256 consecutive rows of one head. Keys come in blocks of
+// 128 from the first key that the first row sees; per tile and block
+//   S = Q K^T        tcgen05.mma 128 x 128 x D, fp32 in TMEM
+//   P = exp2(S c - m) one TMEM lane (query row) per thread, S read once into
+//                    registers, P written back to TMEM as the 16-bit A operand
+//   O += P V         tcgen05.mma 128 x D x 128 accumulating in TMEM, V as it lies in
+//                    memory (MN-major B)
+// While one tile is in the softmax the other one's products run. The maximum m that is
+// subtracted is only raised when a row exceeds it by more than 2^8: P stays below 2^8,
+// the sum is exact to fp32 either way, and O in TMEM is rescaled a few times per row
+// instead of once per block. With D = 64 TMEM holds S, P and O of both tiles apart, so
+// the next S is computed during the softmax; with D = 128 P takes S's columns.
+//
+// Warps 0-3 and 4-7: softmax and output of tile 0 and 1. Warp 8 loads Q, K and V by TMA
+// (128-byte swizzle, K and V blocks in one ring). Warp 9 owns TMEM and issues the MMAs.
+// Every wait is bounded and leaves a code in this file's error word.
+//
+// Bound: with D = 64 the exponentials (one per score, 16 per clock and SM) take twice
+// the tensor time, with D = 128 as long as it.
+#include "../../include/oasis_b200.h"
+#include "attention_prompt.cuh"
+#include "attention_rows.cuh"
+#include "gemm.cuh"
+#include "pages.cuh"
+#include "status.h"
+
+namespace oasis {
+namespace {
+
+constexpr int kTile = 128;  // query rows of a tile, keys of a block
+constexpr int kPromptThreads = 320;
+constexpr float kRaise = 8.f;  // base-2 exponents that a score may exceed the subtracted maximum by
+
+template <int D>
+struct Cfg {
+  static constexpr int CHUNKS = D / 64;               // 64-column chunks: 128 bytes of a row
+  static constexpr int CHUNK_BYTES = kTile * 128;
+  static constexpr int TILE_BYTES = CHUNKS * CHUNK_BYTES;
+  static constexpr int STAGES = D == 64 ? 8 : 5;
+  static constexpr int BAR_BYTES = 512;
+  static constexpr int SMEM = 1024 + (2 + STAGES) * TILE_BYTES + BAR_BYTES;
+  static_assert(SMEM <= 232448, "shared memory");
+  static constexpr bool kApart = D == 64;             // S and P in columns of their own
+  static constexpr int S_COL = 0;                     // + 128 per tile
+  static constexpr int P_COL = kApart ? 256 : 0;      // + P_STEP per tile
+  static constexpr int P_STEP = kApart ? 64 : 128;
+  static constexpr int O_COL = kApart ? 384 : 256;    // + D per tile
+};
+
+__device__ int g_prompt_error = 0;
+
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity, int code) {
+  const uint32_t addr = smem_u32(bar);
+  if (mbar_try_wait(addr, parity)) return true;
+  const long long t0 = clock64();
+  while (!mbar_try_wait(addr, parity)) {
+    if (clock64() - t0 > kWaitClockLimit) {
+      atomicCAS(&g_prompt_error, 0, code);
+      return false;
+    }
+  }
+  return true;
+}
+
+// D[tmem] (+)= A[tmem] * B[smem]
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// V block as an MN-major operand: 64-column chunks CHUNK_BYTES apart (the leading
+// offset), groups of eight keys 1024 bytes apart.
+template <int D>
+__device__ __forceinline__ uint64_t v_desc(uint32_t addr) {
+  return (smem_desc_sw128(addr) & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)(Cfg<D>::CHUNK_BYTES >> 4) << 16);
+}
+
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_16(int n, bool b_mn_major) {
+  return (1u << 4) | (Elem<T>::kHalf ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? 1u << 16 : 0u) |
+         ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+
+// What the block's two tiles cover. Every role works it out alike from cu.
+struct Unit {
+  int head[2], r0[2];       // tile t: its head and first row
+  int begin;                // first key of block 0
+  int first[2], last[2];    // tile t takes key blocks [first, last)
+  int blocks;
+};
+
+__device__ __forceinline__ Unit make_unit(const PromptParams& p, int pair_heads, int end) {
+  Unit u;
+  const int units = pair_heads ? p.heads / 2 : p.heads;
+  const int rows = pair_heads ? kTile : 2 * kTile;
+  const int tiles = (p.rows + rows - 1) / rows;
+  const int x = blockIdx.x % units;
+  const int rt = tiles - 1 - (int)(blockIdx.x / units);  // long key ranges first
+  int low[2];
+  u.begin = 0x7fffffff;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    u.head[t] = pair_heads ? 2 * x + t : x;
+    u.r0[t] = rt * rows + (pair_heads ? 0 : t * kTile);
+    // the first row of the tile that belongs to a sequence, and that sequence's start
+    int lo = 0x7fffffff;
+    if (u.r0[t] < end) {
+      const int i = last_not_above(p.cu, p.n, u.r0[t]);
+      const int a = p.cu[i];
+      if (a > u.r0[t]) {
+        if (a < u.r0[t] + kTile && a < end) lo = a;
+      } else if (a >= 0) {
+        lo = a;
+      }
+    }
+    low[t] = lo;
+    u.begin = min(u.begin, lo);
+  }
+  u.blocks = 0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    u.first[t] = u.last[t] = 0;
+    if (low[t] != 0x7fffffff) {
+      u.first[t] = (low[t] - u.begin) / kTile;
+      u.last[t] = (min(u.r0[t] + kTile, end) - u.begin + kTile - 1) / kTile;
+      u.blocks = max(u.blocks, u.last[t]);
+    }
+  }
+  return u;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+    prompt_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ PromptParams p, int pair_heads) {
+  using C = Cfg<D>;
+  using E = Elem<T>;
+  extern __shared__ uint8_t smem_raw[];
+  pdl_trigger();
+  pdl_wait();
+  const int end = min(p.rows, p.cu[p.n]);
+  const Unit u = make_unit(p, pair_heads, end);
+  if (u.blocks == 0) return;  // the whole block
+
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sKV = sQ + 2 * C::TILE_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + C::STAGES * C::TILE_BYTES);
+  uint64_t* q_full = bars;         // [2]
+  uint64_t* s_full = bars + 2;     // [2]
+  uint64_t* s_read = bars + 4;     // [2] softmax has S in registers (kApart)
+  uint64_t* p_full = bars + 6;     // [2]
+  uint64_t* pv_done = bars + 8;    // [2]
+  uint64_t* drain = bars + 10;
+  uint64_t* kv_full = bars + 16;   // [STAGES <= 8]
+  uint64_t* kv_empty = bars + 24;  // [STAGES <= 8]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&s_read[t], 4);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    mbar_init(drain, 1);
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    fence_barrier_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int kvh0 = u.head[0] / (p.heads / p.kv_heads);
+
+  if (warp == 8) {
+    // ---------------- TMA ----------------
+    if (lane == 0) {
+      auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+        mbar_arrive_expect_tx(bar, C::TILE_BYTES);
+#pragma unroll
+        for (int c = 0; c < C::CHUNKS; ++c) tma_load_3d(dst + c * C::CHUNK_BYTES, map, bar, c * 64, head, row);
+      };
+      const int total = 2 * u.blocks;
+      int issued = 0;
+      bool ok = true;
+      auto next = [&]() {
+        const int st = issued % C::STAGES;
+        if (issued >= C::STAGES && !wait_for(&kv_empty[st], ((issued / C::STAGES) & 1) ^ 1, kDevTimeoutSmemEmpty))
+          return false;
+        load(sKV + st * C::TILE_BYTES, issued & 1 ? &tmV : &tmK, &kv_full[st], kvh0, u.begin + (issued >> 1) * kTile);
+        ++issued;
+        return true;
+      };
+      load(sQ, &tmQ, &q_full[0], u.head[0], u.r0[0]);
+      ok = next();
+      load(sQ + C::TILE_BYTES, &tmQ, &q_full[1], u.head[1], u.r0[1]);
+      while (ok && issued < total) ok = next();
+      if (!ok) {  // gave up: the copies in flight land before the block ends
+        wait_for(&q_full[0], 0, kDevTimeoutTmaFull);
+        wait_for(&q_full[1], 0, kDevTimeoutTmaFull);
+        for (int i = max(0, issued - C::STAGES); i < issued; ++i)
+          wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull);
+      }
+    }
+  } else if (warp == 9) {
+    // ---------------- MMA ----------------
+    if (lane == 0) {
+      constexpr uint32_t idS = idesc_16<T>(kTile, false);
+      constexpr uint32_t idPV = idesc_16<T>(D, true);
+      bool ok = true;
+      auto tile_at_stage = [&](int i) { return smem_u32(sKV + (i % C::STAGES) * C::TILE_BYTES); };
+      auto arrived = [&](int i) { return wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull); };
+      auto release = [&](int i) { tc_commit(&kv_empty[i % C::STAGES]); };
+      auto active = [&](int t, int j) { return j >= u.first[t] && j < u.last[t]; };
+      auto issue_s = [&](int t, int j) {
+        const uint32_t qa = smem_u32(sQ + t * C::TILE_BYTES), ka = tile_at_stage(2 * j);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = (k >> 2) * C::CHUNK_BYTES + (k & 3) * 32;
+          tc_mma_bf16(tmem + C::S_COL + t * kTile, smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), idS, k > 0);
+        }
+        tc_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int t, int j) {
+        const uint32_t va = tile_at_stage(2 * j + 1);
+#pragma unroll
+        for (int k = 0; k < kTile / 16; ++k)
+          mma_ts(tmem + C::O_COL + t * D, tmem + C::P_COL + t * C::P_STEP + k * 8, v_desc<D>(va + k * 2048), idPV,
+                 j > u.first[t] || k > 0);
+        tc_commit(&pv_done[t]);
+      };
+      // the first S of each tile
+      ok = arrived(0);
+      for (int t = 0; t < 2 && ok; ++t)
+        if (active(t, 0)) {
+          ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
+          tc_fence_after();
+          if (ok) issue_s(t, 0);
+        }
+      if (ok) release(0);
+      for (int j = 0; j < u.blocks && ok; ++j) {
+        const bool more = j + 1 < u.blocks;
+        if (more) ok = arrived(2 * (j + 1));
+        if constexpr (C::kApart) {
+          for (int t = 0; t < 2 && ok && more; ++t)
+            if (active(t, j + 1)) {
+              if (j + 1 > u.first[t])
+                ok = wait_for(&s_read[t], (j - u.first[t]) & 1, kDevTimeoutAccEmpty);
+              else
+                ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
+              tc_fence_after();
+              if (ok) issue_s(t, j + 1);
+            }
+          if (ok && more) release(2 * (j + 1));
+        }
+        ok = ok && arrived(2 * j + 1);
+        for (int t = 0; t < 2 && ok; ++t) {
+          if (active(t, j)) {
+            ok = wait_for(&p_full[t], (j - u.first[t]) & 1, kDevTimeoutAccFull);
+            tc_fence_after();
+            if (ok) issue_pv(t, j);
+          }
+          if (!C::kApart && ok && more && active(t, j + 1)) {  // after P V in the same pipe: P's columns are free
+            ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
+            tc_fence_after();
+            if (ok) issue_s(t, j + 1);
+          }
+        }
+        if (ok) {
+          release(2 * j + 1);
+          if (!C::kApart && more) release(2 * (j + 1));
+        }
+      }
+      if (!ok) {
+        tc_commit(drain);
+        wait_for(drain, 0, kDevTimeoutAccFull);
+      }
+    }
+  } else {
+    // ---------------- softmax and output ----------------
+    const int t = warp >> 2, quarter = warp & 3;
+    const int row = u.r0[t] + quarter * 32 + lane;
+    const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_at = lane_base + C::S_COL + t * kTile, p_at = lane_base + C::P_COL + t * C::P_STEP,
+                   o_at = lane_base + C::O_COL + t * D;
+    int lo = row + 1;  // first key that the row sees; row + 1: the row is nobody's
+    if (row < end) {
+      const int i = last_not_above(p.cu, p.n, row);
+      const int a = p.cu[i];
+      if (a >= 0 && a <= row && row < p.cu[i + 1]) lo = a;
+    }
+    const float sc = p.scale_log2;
+    float m = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = u.first[t]; j < u.last[t]; ++j) {
+      const int c = j - u.first[t];
+      if (!wait_for(&s_full[t], c & 1, kDevTimeoutAccFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) tmem_ld32_issue(s_at + x * 32, s[x]);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) tmem_wait_ld(s[x]);
+      if constexpr (C::kApart) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_read[t]);
+      }
+      const int kb = u.begin + j * kTile;
+      if (__any_sync(0xffffffffu, kb < lo || kb + kTile - 1 > row)) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+          for (int k = 0; k < 32; ++k) {
+            const int key = kb + x * 32 + k;
+            if (key < lo || key > row) s[x][k] = 0xff800000u;  // -inf
+          }
+      }
+      float top[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        top[x] = __uint_as_float(s[x][0]);
+#pragma unroll
+        for (int k = 1; k < 32; ++k) top[x] = fmaxf(top[x], __uint_as_float(s[x][k]));
+      }
+      const float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
+      const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
+      float alpha = 1.f;
+      if (raise) {
+        alpha = ex2_approx(m - bm);
+        m = bm;
+        l *= alpha;
+      }
+      const float shift = softmax_shift(m);
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      uint32_t pk[64];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int k = 0; k < 32; k += 2) {
+          const float p0 = ex2_approx(fmaf(__uint_as_float(s[x][k]), sc, -shift));
+          const float p1 = ex2_approx(fmaf(__uint_as_float(s[x][k + 1]), sc, -shift));
+          sum[x] += p0 + p1;
+          pk[x * 16 + k / 2] = E::pack(p0, p1);  // the one rounding inside the sum, half a step per term
+        }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      if (c > 0) {
+        if (!wait_for(&pv_done[t], (c - 1) & 1, kDevTimeoutAccFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int x = 0; x < D / 32; ++x) {
+            uint32_t o[32];
+            tmem_ld32_issue(o_at + x * 32, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+            tmem_st32(o_at + x * 32, o);
+          }
+        }
+      }
+      tmem_st32(p_at, pk);
+      tmem_st32(p_at + 32, pk + 32);
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    const int blocks = u.last[t] - u.first[t];
+    if (ok && blocks > 0 && wait_for(&pv_done[t], (blocks - 1) & 1, kDevTimeoutAccFull)) {
+      tc_fence_after();
+      const bool mine = lo <= row;
+      bool good = l > 0.f && finite_f(l);
+      const float inv = 1.f / l;
+      T* out = static_cast<T*>(p.out) + u.head[t] * p.o_head + row * p.o_row;
+#pragma unroll
+      for (int x = 0; x < D / 32; ++x) {
+        uint32_t o[32];
+        tmem_ld32_issue(o_at + x * 32, o);
+        tmem_wait_ld(o);
+#pragma unroll
+        for (int k = 0; k < 32; ++k) good = good && finite_f(__uint_as_float(o[k]));
+        if (mine) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              w[e] = E::pack(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+            *reinterpret_cast<uint4*>(out + x * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+      unsigned bad = __ballot_sync(0xffffffffu, mine && !good);
+      const T* k0 = static_cast<const T*>(p.k) + kvh0 * p.k_head;
+      const T* v0 = static_cast<const T*>(p.v) + kvh0 * p.v_head;
+      while (bad) {  // rows to be done key by key
+        const int r = __ffs(bad) - 1;
+        bad &= bad - 1;
+        const int at = u.r0[t] + quarter * 32 + r, from = __shfl_sync(0xffffffffu, lo, r);
+        float acc[D / 32] = {}, rm = -INFINITY, rl = 0.f;
+        __syncwarp();  // the row's first result is written
+        row_by_keys<T, D>(
+            static_cast<const T*>(p.q) + u.head[t] * p.q_head + at * p.q_row, sc, at - from + 1,
+            [&](long long x) { return k0 + (from + x) * p.k_row; }, [&](long long x) { return v0 + (from + x) * p.v_row; },
+            acc, rm, rl);
+        T* o = static_cast<T*>(p.out) + u.head[t] * p.o_head + at * p.o_row;
+#pragma unroll
+        for (int d = 0; d < D / 32; d += 2)
+          *reinterpret_cast<uint32_t*>(o + lane * (D / 32) + d) = E::pack(acc[d] / rl, acc[d + 1] / rl);
+      }
+    }
+  }
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 9) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int D>
+int launch(const PromptParams& p, cudaStream_t s) {
+  using C = Cfg<D>;
+  static std::atomic<bool> attr[64];  // per device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    cudaError_t e = cudaFuncSetAttribute(prompt_tc_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+    attr[dev & 63] = true;
+  }
+  const bool half = Elem<T>::kHalf;
+  CUtensorMap tq, tk, tv;
+  OASIS_TRY(make_tma_16bit_3d(&tq, p.q, half, D, p.heads, p.rows, p.q_head, p.q_row, 64, 1, kTile));
+  OASIS_TRY(make_tma_16bit_3d(&tk, p.k, half, D, p.kv_heads, p.rows, p.k_head, p.k_row, 64, 1, kTile));
+  OASIS_TRY(make_tma_16bit_3d(&tv, p.v, half, D, p.kv_heads, p.rows, p.v_head, p.v_row, 64, 1, kTile));
+  const int pair_heads = (p.heads / p.kv_heads) % 2 == 0;
+  const int rows = pair_heads ? kTile : 2 * kTile;
+  const long long blocks = ((long long)p.rows + rows - 1) / rows * (pair_heads ? p.heads / 2 : p.heads);
+  cudaError_t e = launch_pdl(prompt_tc_kernel<T, D>, dim3((unsigned)blocks), dim3(kPromptThreads), C::SMEM, s, tq, tk, tv,
+                             p, pair_heads);
+  if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "prompt_tc_kernel: %s", cudaGetErrorString(e));
+  return check_launch("prompt_tc_kernel");
+}
+
+}  // namespace
+
+int prompt_tc_launch(const PromptParams& p, cudaStream_t s) {
+  if (p.dtype == OASIS_DTYPE_BF16)
+    return p.head_dim == 64 ? launch<__nv_bfloat16, 64>(p, s) : launch<__nv_bfloat16, 128>(p, s);
+  return p.head_dim == 64 ? launch<__half, 64>(p, s) : launch<__half, 128>(p, s);
+}
+
+int read_device_error_prompt(int reset) {
+  int v = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_prompt_error, sizeof(int));
+  if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "device_error: %s", cudaGetErrorString(e));
+  if (reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_prompt_error, &zero, sizeof(int));
+    if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "device_error reset: %s", cudaGetErrorString(e));
+  }
+  return v;
+}
+
+}  // namespace oasis

@@ -1292,6 +1292,23 @@ int make_tma_bf16_2d(CUtensorMap* map, const void* ptr, long long inner, long lo
   return OASIS_OK;
 }
 
+int make_tma_16bit_3d(CUtensorMap* map, const void* ptr, bool half, long long n0, long long n1, long long n2,
+                      long long s1, long long s2, int b0, int b1, int b2) {
+  OASIS_TRY(get_encoder());
+  OASIS_REQUIRE((reinterpret_cast<uintptr_t>(ptr) & 15) == 0, "TMA source not 16-byte aligned");
+  OASIS_REQUIRE(s1 % 8 == 0 && s2 % 8 == 0, "TMA strides not multiples of 16 bytes");
+  cuuint64_t dims[3] = {(cuuint64_t)n0, (cuuint64_t)n1, (cuuint64_t)n2};
+  cuuint64_t strides[2] = {(cuuint64_t)(s1 * 2), (cuuint64_t)(s2 * 2)};
+  cuuint32_t box[3] = {(cuuint32_t)b0, (cuuint32_t)b1, (cuuint32_t)b2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = g_encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(OASIS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return OASIS_OK;
+}
+
 int read_device_error(int reset) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "device_error: %s", cudaGetErrorString(e));

@@ -94,4 +94,9 @@ void set_sm_reserve(int n);
 int make_tma_bf16_2d(CUtensorMap* map, const void* ptr, long long inner, long long outer, long long ld,
                      int box_inner, int box_outer);
 
+// 3-D map of 16-bit elements (fp16 if `half`, else bf16) with the 128-byte swizzle:
+// extents {n0, n1, n2}, element strides {1, s1, s2}, box {b0, b1, b2}; out of range reads 0.
+int make_tma_16bit_3d(CUtensorMap* map, const void* ptr, bool half, long long n0, long long n1, long long n2,
+                      long long s1, long long s2, int b0, int b1, int b2);
+
 }  // namespace oasis
