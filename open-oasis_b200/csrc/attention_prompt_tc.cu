@@ -18,7 +18,9 @@
 // the next S is computed during the softmax; with D = 128 P takes S's columns.
 //
 // Warps 0-3 and 4-7: softmax and output of tile 0 and 1. Warp 8 loads Q, K and V by TMA
-// (128-byte swizzle, K and V blocks in one ring). Warp 9 owns TMEM and issues the MMAs.
+// (128-byte swizzle, K and V blocks in one ring). Warp 9 owns TMEM and issues the MMAs;
+// warps 10 and 11 fill its warpgroup, which gives registers to the other two: 168 per
+// thread at launch become 208, 208 and 88 (a row's 128 scores stay in registers).
 // Every wait is bounded and leaves a code in this file's error word.
 //
 // Bound: with D = 64 the exponentials (one per score, 16 per clock and SM) take twice
@@ -34,7 +36,13 @@ namespace oasis {
 namespace {
 
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
-constexpr int kPromptThreads = 320;
+constexpr int kPromptThreads = 384;
+// Of every eight pairs of exponentials this many go to the FMA pipe, the others to the
+// special-function unit, which alone would be the bound.
+#ifndef OASIS_PROMPT_POLY
+#define OASIS_PROMPT_POLY 2
+#endif
+constexpr int kPoly = OASIS_PROMPT_POLY;
 constexpr float kRaise = 8.f;  // base-2 exponents that a score may exceed the subtracted maximum by
 
 template <int D>
@@ -92,6 +100,61 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Two fp32 values in a register pair: one instruction for both on sm_100.
+__device__ __forceinline__ uint64_t pair2(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 split2(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe, for x <= 8 (values below -125 count as -125):
+// x = n + f with n the nearest whole number (Cody and Waite's reduction: adding
+// 1.5 2^23 leaves n in the low bits), 2^f on [-1/2, 1/2] by the polynomial of least
+// relative error (Remez), n added to the exponent field. Relative error 7.5e-5 in
+// degree 3 for bf16 results (half a step 3.9e-3) and 2.7e-6 in degree 4 for fp16 (4.9e-4).
+template <bool FINE>
+__device__ __forceinline__ float2 exp2_pair(uint64_t x2) {
+  const float2 x = split2(x2);
+  const uint64_t c = pair2(fmaxf(x.x, -125.f), fmaxf(x.y, -125.f));
+  const uint64_t r = add2(c, pair2(12582912.f, 12582912.f));
+  const uint64_t n = add2(r, pair2(-12582912.f, -12582912.f));
+  const uint64_t f = fma2(n, pair2(-1.f, -1.f), c);
+  uint64_t y;
+  if constexpr (FINE) {
+    y = fma2(f, pair2(0.009570102207362652f, 0.009570102207362652f), pair2(0.05591785907745361f, 0.05591785907745361f));
+    y = fma2(f, y, pair2(0.240247443318367f, 0.240247443318367f));
+    y = fma2(f, y, pair2(0.6931217908859253f, 0.6931217908859253f));
+    y = fma2(f, y, pair2(0.9999992847442627f, 0.9999992847442627f));
+  } else {
+    y = fma2(f, pair2(0.0551716685295105f, 0.0551716685295105f), pair2(0.2426111251115799f, 0.2426111251115799f));
+    y = fma2(f, y, pair2(0.6932609677314758f, 0.6932609677314758f));
+    y = fma2(f, y, pair2(0.9999280571937561f, 0.9999280571937561f));
+  }
+  const float2 m = split2(y), b = split2(r);
+  return make_float2(__uint_as_float(__float_as_uint(m.x) + (__float_as_uint(b.x) << 23)),
+                     __uint_as_float(__float_as_uint(m.y) + (__float_as_uint(b.y) << 23)));
+}
+
 // V block as an MN-major operand: 64-column chunks CHUNK_BYTES apart (the leading
 // offset), groups of eight keys 1024 bytes apart.
 template <int D>
@@ -104,6 +167,9 @@ __host__ __device__ constexpr uint32_t idesc_16(int n, bool b_mn_major) {
   return (1u << 4) | (Elem<T>::kHalf ? 0u : (1u << 7) | (1u << 10)) | (b_mn_major ? 1u << 16 : 0u) |
          ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
+
+// A value that all lanes of a warp hold, told to the compiler.
+__device__ __forceinline__ int uniform(int x) { return __shfl_sync(0xffffffffu, x, 0); }
 
 // What the block's two tiles cover. Every role works it out alike from cu.
 struct Unit {
@@ -180,7 +246,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* kv_empty = bars + 24;  // [STAGES <= 8]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
@@ -203,12 +269,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = 0;  // all 512 columns are this block's, so they begin at 0
   const int kvh0 = u.head[0] / (p.heads / p.kv_heads);
 
-  if (warp == 8) {
-    // ---------------- TMA ----------------
-    if (lane == 0) {
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
+    if (warp == 8 && lane == 0) {
+      // ---------------- TMA ----------------
       auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
         mbar_arrive_expect_tx(bar, C::TILE_BYTES);
 #pragma unroll
@@ -236,67 +303,84 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull);
       }
     }
-  } else if (warp == 9) {
-    // ---------------- MMA ----------------
-    if (lane == 0) {
+    if (warp == 9) {
+      // ---------------- MMA ----------------
+      // The whole warp walks the loop with values that are the same in all lanes, so
+      // that descriptors live in uniform registers, and one elected lane issues: from
+      // a single-lane branch each tcgen05.mma took about 100 cycles to issue (D = 64,
+      // 24 of them a block pair), more than the 32 to 64 that it runs.
       constexpr uint32_t idS = idesc_16<T>(kTile, false);
       constexpr uint32_t idPV = idesc_16<T>(D, true);
+      const bool one = elect_one();
+      const int blocks = uniform(u.blocks);
+      const int first[2] = {uniform(u.first[0]), uniform(u.first[1])}, last[2] = {uniform(u.last[0]), uniform(u.last[1])};
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ)), k_desc = smem_desc_sw128(smem_u32(sKV)),
+                     v_desc0 = v_desc<D>(smem_u32(sKV));
       bool ok = true;
-      auto tile_at_stage = [&](int i) { return smem_u32(sKV + (i % C::STAGES) * C::TILE_BYTES); };
-      auto arrived = [&](int i) { return wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull); };
-      auto release = [&](int i) { tc_commit(&kv_empty[i % C::STAGES]); };
-      auto active = [&](int t, int j) { return j >= u.first[t] && j < u.last[t]; };
+      auto wait_all = [&](uint64_t* bar, uint32_t parity, int code) {
+        return __all_sync(0xffffffffu, wait_for(bar, parity, code)) != 0;
+      };
+      auto stage_off = [&](int i) { return (uint64_t)(i % C::STAGES * (C::TILE_BYTES >> 4)); };
+      auto arrived = [&](int i) { return wait_all(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull); };
+      auto release = [&](int i) {
+        if (one) tc_commit(&kv_empty[i % C::STAGES]);
+      };
+      auto active = [&](int t, int j) { return j >= first[t] && j < last[t]; };
       auto issue_s = [&](int t, int j) {
-        const uint32_t qa = smem_u32(sQ + t * C::TILE_BYTES), ka = tile_at_stage(2 * j);
+        tc_fence_after();
+        const uint64_t qa = q_desc + (uint64_t)(t * (C::TILE_BYTES >> 4)), ka = k_desc + stage_off(2 * j);
+        if (one) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t off = (k >> 2) * C::CHUNK_BYTES + (k & 3) * 32;
-          tc_mma_bf16(tmem + C::S_COL + t * kTile, smem_desc_sw128(qa + off), smem_desc_sw128(ka + off), idS, k > 0);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = ((k >> 2) * C::CHUNK_BYTES + (k & 3) * 32) >> 4;
+            tc_mma_bf16(C::S_COL + t * kTile, qa + off, ka + off, idS, k > 0);
+          }
+          tc_commit(&s_full[t]);
         }
-        tc_commit(&s_full[t]);
       };
       auto issue_pv = [&](int t, int j) {
-        const uint32_t va = tile_at_stage(2 * j + 1);
+        tc_fence_after();
+        const uint64_t va = v_desc0 + stage_off(2 * j + 1);
+        const uint32_t more = j > first[t];
+        if (one) {
 #pragma unroll
-        for (int k = 0; k < kTile / 16; ++k)
-          mma_ts(tmem + C::O_COL + t * D, tmem + C::P_COL + t * C::P_STEP + k * 8, v_desc<D>(va + k * 2048), idPV,
-                 j > u.first[t] || k > 0);
-        tc_commit(&pv_done[t]);
+          for (int k = 0; k < kTile / 16; ++k)
+            mma_ts(C::O_COL + t * D, C::P_COL + t * C::P_STEP + k * 8, va + (uint64_t)(k * 2048 >> 4), idPV,
+                   k > 0 ? 1u : more);
+          tc_commit(&pv_done[t]);
+        }
       };
       // the first S of each tile
       ok = arrived(0);
-      for (int t = 0; t < 2 && ok; ++t)
-        if (active(t, 0)) {
-          ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
-          tc_fence_after();
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (ok && active(t, 0)) {
+          ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
           if (ok) issue_s(t, 0);
         }
       if (ok) release(0);
-      for (int j = 0; j < u.blocks && ok; ++j) {
-        const bool more = j + 1 < u.blocks;
+      for (int j = 0; j < blocks && ok; ++j) {
+        const bool more = j + 1 < blocks;
         if (more) ok = arrived(2 * (j + 1));
         if constexpr (C::kApart) {
-          for (int t = 0; t < 2 && ok && more; ++t)
-            if (active(t, j + 1)) {
-              if (j + 1 > u.first[t])
-                ok = wait_for(&s_read[t], (j - u.first[t]) & 1, kDevTimeoutAccEmpty);
-              else
-                ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
-              tc_fence_after();
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            if (ok && more && active(t, j + 1)) {
+              ok = j + 1 > first[t] ? wait_all(&s_read[t], (j - first[t]) & 1, kDevTimeoutAccEmpty)
+                                    : wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
               if (ok) issue_s(t, j + 1);
             }
           if (ok && more) release(2 * (j + 1));
         }
         ok = ok && arrived(2 * j + 1);
-        for (int t = 0; t < 2 && ok; ++t) {
-          if (active(t, j)) {
-            ok = wait_for(&p_full[t], (j - u.first[t]) & 1, kDevTimeoutAccFull);
-            tc_fence_after();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (ok && active(t, j)) {
+            ok = wait_all(&p_full[t], (j - first[t]) & 1, kDevTimeoutAccFull);
             if (ok) issue_pv(t, j);
           }
           if (!C::kApart && ok && more && active(t, j + 1)) {  // after P V in the same pipe: P's columns are free
-            ok = wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
-            tc_fence_after();
+            ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
             if (ok) issue_s(t, j + 1);
           }
         }
@@ -306,23 +390,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       if (!ok) {
-        tc_commit(drain);
+        if (one) tc_commit(drain);
         wait_for(drain, 0, kDevTimeoutAccFull);
       }
     }
   } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------- softmax and output ----------------
     const int t = warp >> 2, quarter = warp & 3;
     const int row = u.r0[t] + quarter * 32 + lane;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_at = lane_base + C::S_COL + t * kTile, p_at = lane_base + C::P_COL + t * C::P_STEP,
                    o_at = lane_base + C::O_COL + t * D;
-    int lo = row + 1;  // first key that the row sees; row + 1: the row is nobody's
+    int lo = 0x3fffffff;  // first key that the row sees; beyond all keys where the row is nobody's
     if (row < end) {
       const int i = last_not_above(p.cu, p.n, row);
       const int a = p.cu[i];
       if (a >= 0 && a <= row && row < p.cu[i + 1]) lo = a;
     }
+    const unsigned span = lo <= row ? row - lo : 0;  // sees keys lo .. lo + span
     const float sc = p.scale_log2;
     float m = -INFINITY, l = 0.f;
     bool ok = true;
@@ -348,17 +434,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const int key = kb + x * 32 + k;
-            if (key < lo || key > row) s[x][k] = 0xff800000u;  // -inf
-          }
+          for (int k = 0; k < 32; ++k)
+            if ((unsigned)(kb - lo + x * 32 + k) > span) s[x][k] = 0xff800000u;  // -inf
       }
       float top[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        top[x] = __uint_as_float(s[x][0]);
+        top[x] = fmaxf(__uint_as_float(s[x][0]), __uint_as_float(s[x][1]));
 #pragma unroll
-        for (int k = 1; k < 32; ++k) top[x] = fmaxf(top[x], __uint_as_float(s[x][k]));
+        for (int k = 2; k < 32; k += 2) top[x] = max3(top[x], __uint_as_float(s[x][k]), __uint_as_float(s[x][k + 1]));
       }
       const float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
       const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
@@ -369,18 +453,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         l *= alpha;
       }
       const float shift = softmax_shift(m);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t sc2 = pair2(sc, sc), shift2 = pair2(-shift, -shift);
+      uint64_t sum[4] = {0, 0, 0, 0};
       uint32_t pk[64];
 #pragma unroll
       for (int x = 0; x < 4; ++x)
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
-          const float p0 = ex2_approx(fmaf(__uint_as_float(s[x][k]), sc, -shift));
-          const float p1 = ex2_approx(fmaf(__uint_as_float(s[x][k + 1]), sc, -shift));
-          sum[x] += p0 + p1;
-          pk[x * 16 + k / 2] = E::pack(p0, p1);  // the one rounding inside the sum, half a step per term
+          const uint64_t e = fma2(pair2(__uint_as_float(s[x][k]), __uint_as_float(s[x][k + 1])), sc2, shift2);
+          float2 y;
+          if ((k / 2) % 8 < kPoly) {
+            y = exp2_pair<E::kHalf>(e);
+          } else {
+            y = split2(e);
+            y = make_float2(ex2_approx(y.x), ex2_approx(y.y));
+          }
+          sum[x] = add2(sum[x], pair2(y.x, y.y));
+          pk[x * 16 + k / 2] = E::pack(y.x, y.y);  // the one rounding inside the sum, half a step per term
         }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float2 part = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
+      l += part.x + part.y;
       if (c > 0) {
         if (!wait_for(&pv_done[t], (c - 1) & 1, kDevTimeoutAccFull)) {
           ok = false;
@@ -410,7 +502,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     if (ok && blocks > 0 && wait_for(&pv_done[t], (blocks - 1) & 1, kDevTimeoutAccFull)) {
       tc_fence_after();
       const bool mine = lo <= row;
-      bool good = l > 0.f && finite_f(l);
+      bool good = l > 0.f && finite_f(l) && m != -INFINITY;
       const float inv = 1.f / l;
       T* out = static_cast<T*>(p.out) + u.head[t] * p.o_head + row * p.o_row;
 #pragma unroll
@@ -455,7 +547,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == 9) tmem_dealloc(tmem, 512);
+  if (warp == 9) tmem_dealloc(*tmem_slot, 512);
 }
 
 template <typename T, int D>

@@ -190,11 +190,13 @@ def error_bound(want, spread, reach, keys, D, dtype):
     (u); a score's sum of D products and its scaling (D + 4 roundings of 2^-24 of
     `reach`), the maximum subtracted in the base-2 exponent (4 more), a probability
     that is exp(score) moved by as much, in the sum and in the total (twice); the
-    exponential's own 2^-21 twice; the sums over keys (keys 2^-24 twice). `tiny`: what
+    exponential's own error twice (2^-21 from the special-function unit, 2^-13.7 for bf16
+    and 2^-18.4 for fp16 where a polynomial takes its place: the measured maxima of the
+    two polynomials over their interval); the sums over keys (keys 2^-24 twice). `tiny`: what
     underflows (probabilities below 2^-25 of the largest in fp16, results below the
     smallest step)."""
     u = torch.finfo(dtype).eps / 2
-    drift = 2 * ((D + 8) * reach * 1.4427 + 2 * keys) * 2.0 ** -24 + 2.0 ** -20
+    drift = 2 * ((D + 8) * reach * 1.4427 + 2 * keys) * 2.0 ** -24 + 2 * 2.0 ** (-18.4 if dtype == torch.float16 else -13.7)
     tiny = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -120
     rel = (1 + u) * (1 + drift) * (1 + u) - 1
     return (rel * spread + u * want.abs()) * 1.0001 + tiny * (1 + keys * (dtype == torch.float16) * 2)
