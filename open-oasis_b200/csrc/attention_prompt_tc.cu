@@ -18,8 +18,8 @@
 // the next S is computed during the softmax; with D = 128 P takes S's columns.
 //
 // Warps 0-3 and 4-7: softmax and output of tile 0 and 1. Warp 8 loads Q, K and V by TMA
-// (128-byte swizzle, K and V blocks in one ring). Warp 9 owns TMEM and issues the MMAs;
-// warps 10 and 11 fill its warpgroup, which gives registers to the other two: 168 per
+// (128-byte swizzle, K and V blocks in one ring). Warps 9 and 10 (D = 128: 9 alone) issue
+// the MMAs, warp 9 owns TMEM. Their warpgroup gives registers to the other two: 168 per
 // thread at launch become 208, 208 and 88 (a row's 128 scores stay in registers).
 // Every wait is bounded and leaves a code in this file's error word.
 //
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   uint64_t* s_read = bars + 4;     // [2] softmax has S in registers (kApart)
   uint64_t* p_full = bars + 6;     // [2]
   uint64_t* pv_done = bars + 8;    // [2]
-  uint64_t* drain = bars + 10;
+  uint64_t* drain = bars + 10;     // [2]
   uint64_t* kv_full = bars + 16;   // [STAGES <= 8]
   uint64_t* kv_empty = bars + 24;  // [STAGES <= 8]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
@@ -254,11 +254,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       mbar_init(&s_read[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&pv_done[t], 1);
+      mbar_init(&drain[t], 1);
     }
-    mbar_init(drain, 1);
     for (int i = 0; i < C::STAGES; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], C::kApart ? 2 : 1);
     }
     fence_barrier_init();
   }
@@ -303,15 +303,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull);
       }
     }
-    if (warp == 9) {
+    if (warp == 9 || (C::kApart && warp == 10)) {
       // ---------------- MMA ----------------
+      // D = 64: a warp per tile; with one warp for both, issuing 24 MMAs and waiting
+      // for six barriers in turn took as long as the softmax. D = 128: one warp, so
+      // that a tile's P V and next S run one behind the other and the tiles take turns;
+      // issued by two warps they mixed and both tiles waited for all four.
       // The whole warp walks the loop with values that are the same in all lanes, so
       // that descriptors live in uniform registers, and one elected lane issues: from
-      // a single-lane branch each tcgen05.mma took about 100 cycles to issue (D = 64,
-      // 24 of them a block pair), more than the 32 to 64 that it runs.
+      // a single-lane branch each tcgen05.mma took about 100 cycles to issue.
       constexpr uint32_t idS = idesc_16<T>(kTile, false);
       constexpr uint32_t idPV = idesc_16<T>(D, true);
       const bool one = elect_one();
+      const int t0 = warp - 9, t1 = C::kApart ? t0 + 1 : 2;  // this warp's tiles
       const int blocks = uniform(u.blocks);
       const int first[2] = {uniform(u.first[0]), uniform(u.first[1])}, last[2] = {uniform(u.last[0]), uniform(u.last[1])};
       const uint64_t q_desc = smem_desc_sw128(smem_u32(sQ)), k_desc = smem_desc_sw128(smem_u32(sKV)),
@@ -322,6 +326,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       };
       auto stage_off = [&](int i) { return (uint64_t)(i % C::STAGES * (C::TILE_BYTES >> 4)); };
       auto arrived = [&](int i) { return wait_all(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull); };
+      // K or V block i, which has arrived, is not needed by this warp any more once the
+      // MMAs issued so far are done
       auto release = [&](int i) {
         if (one) tc_commit(&kv_empty[i % C::STAGES]);
       };
@@ -329,11 +335,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       auto issue_s = [&](int t, int j) {
         tc_fence_after();
         const uint64_t qa = q_desc + (uint64_t)(t * (C::TILE_BYTES >> 4)), ka = k_desc + stage_off(2 * j);
+        const uint32_t d = C::S_COL + t * kTile;
         if (one) {
 #pragma unroll
           for (int k = 0; k < D / 16; ++k) {
             const uint64_t off = ((k >> 2) * C::CHUNK_BYTES + (k & 3) * 32) >> 4;
-            tc_mma_bf16(C::S_COL + t * kTile, qa + off, ka + off, idS, k > 0);
+            tc_mma_bf16(d, qa + off, ka + off, idS, k > 0);
           }
           tc_commit(&s_full[t]);
         }
@@ -341,48 +348,36 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       auto issue_pv = [&](int t, int j) {
         tc_fence_after();
         const uint64_t va = v_desc0 + stage_off(2 * j + 1);
-        const uint32_t more = j > first[t];
+        const uint32_t more = j > first[t], d = C::O_COL + t * D, pa = C::P_COL + t * C::P_STEP;
         if (one) {
 #pragma unroll
-          for (int k = 0; k < kTile / 16; ++k)
-            mma_ts(C::O_COL + t * D, C::P_COL + t * C::P_STEP + k * 8, va + (uint64_t)(k * 2048 >> 4), idPV,
-                   k > 0 ? 1u : more);
+          for (int k = 0; k < kTile / 16; ++k) mma_ts(d, pa + k * 8, va + (uint64_t)(k * 2048 >> 4), idPV, k > 0 ? 1u : more);
           tc_commit(&pv_done[t]);
         }
       };
-      // the first S of each tile
+      auto next_s = [&](int t, int j) {  // K block j has arrived
+        if (!ok || !active(t, j)) return;
+        if (j == first[t]) ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
+        if (ok && C::kApart && j > first[t]) ok = wait_all(&s_read[t], (j - 1 - first[t]) & 1, kDevTimeoutAccEmpty);
+        if (ok) issue_s(t, j);
+      };
       ok = arrived(0);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (ok && active(t, 0)) {
-          ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
-          if (ok) issue_s(t, 0);
-        }
+      for (int t = t0; t < t1; ++t) next_s(t, 0);
       if (ok) release(0);
       for (int j = 0; j < blocks && ok; ++j) {
         const bool more = j + 1 < blocks;
         if (more) ok = arrived(2 * (j + 1));
-        if constexpr (C::kApart) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            if (ok && more && active(t, j + 1)) {
-              ok = j + 1 > first[t] ? wait_all(&s_read[t], (j - first[t]) & 1, kDevTimeoutAccEmpty)
-                                    : wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
-              if (ok) issue_s(t, j + 1);
-            }
-          if (ok && more) release(2 * (j + 1));
+        if (C::kApart && more) {
+          next_s(t0, j + 1);
+          if (ok) release(2 * (j + 1));
         }
         ok = ok && arrived(2 * j + 1);
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = t0; t < t1; ++t) {
           if (ok && active(t, j)) {
             ok = wait_all(&p_full[t], (j - first[t]) & 1, kDevTimeoutAccFull);
             if (ok) issue_pv(t, j);
           }
-          if (!C::kApart && ok && more && active(t, j + 1)) {  // after P V in the same pipe: P's columns are free
-            ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
-            if (ok) issue_s(t, j + 1);
-          }
+          if (!C::kApart && more) next_s(t, j + 1);  // behind P V in the same pipe: P's columns are free
         }
         if (ok) {
           release(2 * j + 1);
@@ -390,8 +385,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         }
       }
       if (!ok) {
-        if (one) tc_commit(drain);
-        wait_for(drain, 0, kDevTimeoutAccFull);
+        if (one) tc_commit(&drain[t0]);
+        wait_for(&drain[t0], 0, kDevTimeoutAccFull);
       }
     }
   } else {
@@ -444,20 +439,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
 #pragma unroll
         for (int k = 2; k < 32; k += 2) top[x] = max3(top[x], __uint_as_float(s[x][k]), __uint_as_float(s[x][k + 1]));
       }
-      const float bm = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * sc;
-      const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
-      float alpha = 1.f;
-      if (raise) {
-        alpha = ex2_approx(m - bm);
-        m = bm;
-        l *= alpha;
-      }
-      const float shift = softmax_shift(m);
-      const uint64_t sc2 = pair2(sc, sc), shift2 = pair2(-shift, -shift);
-      uint64_t sum[4] = {0, 0, 0, 0};
+      const float bm = max3(fmaxf(top[0], top[1]), top[2], top[3]) * sc;
+      uint64_t sum[4];
       uint32_t pk[64];
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
+      const uint64_t sc2 = pair2(sc, sc);
+      auto quarter_of_p = [&](int x, float shift) {
+        const uint64_t shift2 = pair2(-shift, -shift);
+        sum[x] = 0;
 #pragma unroll
         for (int k = 0; k < 32; k += 2) {
           const uint64_t e = fma2(pair2(__uint_as_float(s[x][k]), __uint_as_float(s[x][k + 1])), sc2, shift2);
@@ -471,6 +459,29 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           sum[x] = add2(sum[x], pair2(y.x, y.y));
           pk[x * 16 + k / 2] = E::pack(y.x, y.y);  // the one rounding inside the sum, half a step per term
         }
+      };
+      const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
+      const bool any_raise = __any_sync(0xffffffffu, raise);
+      float alpha = 1.f;
+      if (raise) {
+        alpha = ex2_approx(m - bm);
+        m = bm;
+        l *= alpha;
+      }
+      auto rescale = [&]() {  // O of the blocks so far, whose P V is done
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+          uint32_t o[32];
+          tmem_ld32_issue(o_at + x * 32, o);
+          tmem_wait_ld(o);
+#pragma unroll
+          for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+          tmem_st32(o_at + x * 32, o);
+        }
+      };
+      const float shift = softmax_shift(m);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) quarter_of_p(x, shift);
       const float2 part = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
       l += part.x + part.y;
       if (c > 0) {
@@ -479,17 +490,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           break;
         }
         tc_fence_after();
-        if (__any_sync(0xffffffffu, raise)) {
-#pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            uint32_t o[32];
-            tmem_ld32_issue(o_at + x * 32, o);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-            tmem_st32(o_at + x * 32, o);
-          }
-        }
+        if (any_raise) rescale();
       }
       tmem_st32(p_at, pk);
       tmem_st32(p_at + 32, pk + 32);
