@@ -179,13 +179,9 @@ struct Unit {
   int blocks;
 };
 
-__device__ __forceinline__ Unit make_unit(const PromptParams& p, int pair_heads, int end) {
+__device__ __forceinline__ Unit make_unit(const PromptParams& p, int pair_heads, int end, int x, int rt) {
   Unit u;
-  const int units = pair_heads ? p.heads / 2 : p.heads;
   const int rows = pair_heads ? kTile : 2 * kTile;
-  const int tiles = (p.rows + rows - 1) / rows;
-  const int x = blockIdx.x % units;
-  const int rt = tiles - 1 - (int)(blockIdx.x / units);  // long key ranges first
   int low[2];
   u.begin = 0x7fffffff;
 #pragma unroll
@@ -194,9 +190,10 @@ __device__ __forceinline__ Unit make_unit(const PromptParams& p, int pair_heads,
     u.r0[t] = rt * rows + (pair_heads ? 0 : t * kTile);
     // the first row of the tile that belongs to a sequence, and that sequence's start
     int lo = 0x7fffffff;
-    if (u.r0[t] < end) {
-      const int i = last_not_above(p.cu, p.n, u.r0[t]);
-      const int a = p.cu[i];
+    if (t == 1 && pair_heads) {
+      lo = low[0];
+    } else if (u.r0[t] < end) {
+      const int a = p.cu[last_not_above(p.cu, p.n, u.r0[t])];
       if (a > u.r0[t]) {
         if (a < u.r0[t] + kTile && a < end) lo = a;
       } else if (a >= 0) {
@@ -229,7 +226,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   pdl_trigger();
   pdl_wait();
   const int end = min(p.rows, p.cu[p.n]);
-  const Unit u = make_unit(p, pair_heads, end);
+  // Work: a row tile (pair) x a head (pair), the last rows first: in a sequence those
+  // see the most keys, and the blocks that finish last should be short.
+  const int head_units = pair_heads ? p.heads / 2 : p.heads;
+  const int tile_rows = pair_heads ? kTile : 2 * kTile;
+  const int at = blockIdx.x / head_units;
+  const Unit u = make_unit(p, pair_heads, end, blockIdx.x - at * head_units, (p.rows + tile_rows - 1) / tile_rows - 1 - at);
   if (u.blocks == 0) return;  // the whole block
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -505,7 +507,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
       const bool mine = lo <= row;
       bool good = l > 0.f && finite_f(l) && m != -INFINITY;
       const float inv = 1.f / l;
-      T* out = static_cast<T*>(p.out) + u.head[t] * p.o_head + row * p.o_row;
+      // Through this tile's Q, which no product reads any more, so that a store covers
+      // four rows' 128 bytes: a thread per row writing its own 16 bytes at a time
+      // touched 32 lines a store and took 2 to 3.5 us a tile.
+      const unsigned mine_rows = __ballot_sync(0xffffffffu, mine);
+      uint8_t* stage = sQ + t * C::TILE_BYTES + quarter * (32 * 128);
+      T* out = static_cast<T*>(p.out) + u.head[t] * p.o_head + (long long)(u.r0[t] + quarter * 32) * p.o_row;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
@@ -513,15 +520,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         tmem_wait_ld(o);
 #pragma unroll
         for (int k = 0; k < 32; ++k) good = good && finite_f(__uint_as_float(o[k]));
-        if (mine) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t w[4];
+        for (int q = 0; q < 4; ++q) {
+          uint32_t w[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = E::pack(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(out + x * 32 + q * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int e = 0; e < 4; ++e)
+            w[e] = E::pack(__uint_as_float(o[8 * q + 2 * e]) * inv, __uint_as_float(o[8 * q + 2 * e + 1]) * inv);
+          *reinterpret_cast<uint4*>(stage + tile_at<64>(lane, (x & 1) * 4 + q)) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (x & 1) {
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int r = i * 4 + (lane >> 3), ch = lane & 7;
+            const uint4 y = *reinterpret_cast<const uint4*>(stage + tile_at<64>(r, ch));
+            if (mine_rows >> r & 1) *reinterpret_cast<uint4*>(out + r * p.o_row + (x >> 1) * 64 + ch * 8) = y;
           }
+          __syncwarp();
         }
       }
       unsigned bad = __ballot_sync(0xffffffffu, mine && !good);
