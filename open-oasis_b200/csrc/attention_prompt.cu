@@ -20,7 +20,13 @@
 namespace oasis {
 namespace {
 
-constexpr int kRowsTile = 64;  // query rows of a block, and keys of a step
+constexpr int kRowsTile = 64;   // query rows of a block
+// Keys of a step. The first step's are the tile's own rows and 16 before them: they are
+// loaded before it is known which sequences the rows belong to, and sequences of up to
+// 17 tokens need no other. Further steps go back from there. One buffer: what hides the
+// loads is the other blocks of the SM.
+constexpr int kRowsBefore = 16;
+constexpr int kRowsKeys = kRowsTile + kRowsBefore;
 constexpr int kRowsThreads = 128;
 
 // Up to this length the rows kernel is taken.
@@ -28,62 +34,81 @@ constexpr int kShort = 64;
 
 template <int D>
 constexpr int rows_smem() {
-  return 5 * kRowsTile * D * 2;  // Q (then O), two K and two V tiles
+  return (kRowsTile + 2 * kRowsKeys) * D * 2;  // Q (then O), K and V
 }
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(PromptParams p) {
+__global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_kernel(PromptParams p) {
   using E = Elem<T>;
   constexpr int CH = D / 8;   // 16-byte chunks of a row
   constexpr int KS = D / 16;  // k steps of Q K^T
   constexpr int NT = D / 8;   // 8-wide column tiles of O
-  constexpr int TILE = kRowsTile * D * 2;
+  constexpr int Q_BYTES = kRowsTile * D * 2, K_BYTES = kRowsKeys * D * 2;
   extern __shared__ __align__(128) uint8_t sm[];
   __shared__ int first[kRowsTile];  // first key that a row sees; row + 1 where the row is nobody's
   __shared__ int lowest[2];
+  __shared__ int starts[kRowsThreads];  // offsets from the first row's sequence on
   pdl_trigger();
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int head = blockIdx.x % p.heads, r0 = (int)(blockIdx.x / p.heads) * kRowsTile;
-  const int end = min(p.rows, p.cu[p.n]);
-  if (r0 >= end) return;
   const T* q = static_cast<const T*>(p.q) + head * p.q_head;
   const int kvh = head / (p.heads / p.kv_heads);
   const T* k = static_cast<const T*>(p.k) + kvh * p.k_head;
   const T* v = static_cast<const T*>(p.v) + kvh * p.v_head;
 
+  uint8_t* const sk = sm + Q_BYTES;
+  uint8_t* const sv = sk + K_BYTES;
   for (int x = tid; x < kRowsTile * CH; x += kRowsThreads) {
     const int r = x / CH, c = x % CH;
-    const bool ok = r0 + r < end;
+    const bool ok = r0 + r < p.rows;
     cp_async16(sm + tile_at<D>(r, c), q + (ok ? r0 + r : 0) * p.q_row + c * 8, ok);
   }
+  auto load = [&](int at) {
+    for (int x = tid; x < kRowsKeys * CH; x += kRowsThreads) {
+      const int r = x / CH, c = x % CH;
+      const bool ok = at + r >= 0 && at + r < p.rows;
+      const long long row = ok ? at + r : 0;
+      cp_async16(sk + tile_at<D>(r, c), k + row * p.k_row + c * 8, ok);
+      cp_async16(sv + tile_at<D>(r, c), v + row * p.v_row + c * 8, ok);
+    }
+  };
+  load(r0 - kRowsBefore);
+  const int end = min(p.rows, p.cu[p.n]);
+  if (r0 >= end) {
+    cp_async_wait_all();
+    return;
+  }
+  // The first row's sequence, a warp probing 32 places at a time; the other rows of the
+  // tile belong to it or to the ones behind it.
+  int i0 = 0;
+  for (int n = p.n; n > 1;) {
+    const int step = (n + 31) / 32;
+    const int i = lane * step;
+    const bool ok = i < n && p.cu[i0 + i] <= r0;
+    const int c = 32 - __clz(__ballot_sync(0xffffffffu, ok) | 1u);  // probes that hold: a run from lane 0
+    i0 += (c - 1) * step;
+    n = min(step, n - (c - 1) * step);
+  }
+  starts[tid] = p.cu[min(i0 + tid, p.n)];
+  __syncthreads();
   if (tid < kRowsTile) {
     const int r = r0 + tid;
-    const int i = last_not_above(p.cu, p.n, r);
-    const int a = p.cu[i];
-    const bool mine = r < end && a >= 0 && a <= r && r < p.cu[i + 1];
+    const int k = last_not_above(starts, kRowsThreads, r);
+    int i = i0 + k, a = starts[k];
+    int b = k + 1 < kRowsThreads ? starts[k + 1] : 0;
+    if (k + 1 == kRowsThreads || i >= p.n) {  // behind the offsets at hand, or the last row's
+      i = last_not_above(p.cu, p.n, r);
+      a = p.cu[i];
+      b = p.cu[i + 1];
+    }
+    const bool mine = r < end && a >= 0 && a <= r && r < b;
     first[tid] = mine ? a : r + 1;
     const int low = __reduce_min_sync(0xffffffffu, first[tid]);
     if (lane == 0) lowest[warp] = low;
   }
   __syncthreads();
   const int k_begin = min(lowest[0], lowest[1]);
-  const int k_end = min(r0 + kRowsTile, end);
-  const int steps = k_end > k_begin ? (k_end - k_begin + kRowsTile - 1) / kRowsTile : 0;
-  auto load = [&](int j) {
-    uint8_t* kd = sm + TILE + (j & 1) * 2 * TILE;
-    const int at = k_begin + j * kRowsTile;
-    for (int x = tid; x < kRowsTile * CH; x += kRowsThreads) {
-      const int r = x / CH, c = x % CH;
-      const bool ok = at + r < k_end;
-      const long long row = ok ? at + r : 0;
-      cp_async16(kd + tile_at<D>(r, c), k + row * p.k_row + c * 8, ok);
-      cp_async16(kd + TILE + tile_at<D>(r, c), v + row * p.v_row + c * 8, ok);
-    }
-    cp_async_commit();
-  };
-  if (steps > 0) load(0);
-
   const int wr = warp * 16;  // this warp's first row in the tile
   const int ra = wr + (lane >> 2), rb = ra + 8;
   const int lo_a = first[ra], lo_b = first[rb];
@@ -94,24 +119,20 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(PromptParams 
   for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
 
-  for (int j = 0; j < steps; ++j) {
-    if (j + 1 < steps) {
-      load(j + 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
+  for (int at = r0 - kRowsBefore, j = 0; j == 0 || at + kRowsKeys > k_begin; at -= kRowsKeys, ++j) {
+    if (j) {
+      __syncthreads();  // the keys before are done with
+      load(at);
     }
+    cp_async_wait_all();
     __syncthreads();
     if (j == 0) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
     }
-    const int at = k_begin + j * kRowsTile;
-    const uint8_t* sk = sm + TILE + (j & 1) * 2 * TILE;
-    const uint8_t* sv = sk + TILE;
     // 16 keys at a time: the visible range of this warp's rows is [low, r0 + wr + 15]
 #pragma unroll
-    for (int h = 0; h < kRowsTile / 16; ++h) {
+    for (int h = 0; h < kRowsKeys / 16; ++h) {
       const int kb = at + h * 16;
       if (kb > r0 + wr + 15 || kb + 15 < low) continue;
       float x[2][4] = {};
@@ -170,9 +191,7 @@ __global__ void __launch_bounds__(kRowsThreads) prompt_rows_kernel(PromptParams 
         }
       }
     }
-    __syncthreads();  // the tile may be overwritten
   }
-  cp_async_wait_all();  // a tile without keys has only Q in flight
 #pragma unroll
   for (int w = 1; w < 4; w <<= 1) {
     la += __shfl_xor_sync(0xffffffffu, la, w);
