@@ -37,7 +37,7 @@ struct SharedParams {
   float* part_o;   // [rows heads][splits][D]
   float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
   int rows, groups, heads, per, layer;  // per: heads of a key head
-  int prefix_splits, own_splits, tiles, head_tiles;
+  int prefix_splits, own_splits, tiles, head_tiles, whole;
   float scale_log2;
 };
 
@@ -494,6 +494,284 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     if (bad >> r & 1) row_again<T, D>(p, b, h0 + r);
 }
 
+// Prefix and own keys in one pass, for many rows with few keys each (forks of a short
+// prompt: a group per patch, a few frames behind it): 64 (row, head) queries of one key
+// head per block, whatever groups they belong to. Each group's prefix is read once for
+// the rows of the tile that are in it, then each warp goes through the own keys of its
+// 16 queries' rows, 16 keys at a time: the product is taken with all 16 queries and the
+// other rows' scores are masked, so that the softmax and O stay in one fragment and
+// nothing goes through memory in between.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel(SharedParams p) {
+  constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kPrefixKeys * D * 2, UNIT = kUnit * D * 2;
+  extern __shared__ __align__(128) uint8_t sm[];
+  __shared__ int row_of[kPrefixRows];    // row of a query, -1: none
+  __shared__ int seq_of[kPrefixRows];    // its sequence
+  __shared__ int len_of[kPrefixRows];    // its tokens
+  __shared__ int begin_of[kPrefixRows];  // its first own token
+  __shared__ int group_of[kPrefixRows];
+  __shared__ int near_starts[kThreads];  // group starts from the first query's group on
+  __shared__ int lead_len[4], lead_row[4];
+  __shared__ int unit_ok[2][4];
+  pdl_trigger();
+  pdl_wait();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int kvh = blockIdx.x % p.g.kv_heads;
+  const long long m0 = (long long)(blockIdx.x / p.g.kv_heads) * kPrefixRows, queries = (long long)p.rows * p.per;
+  const int P = p.g.page_size;
+  const uint4* pool = static_cast<const uint4*>(p.pool);
+  const long long to_v = p.g.kv_heads * tile_vectors(p.g);
+  const T* q = static_cast<const T*>(p.q);
+  for (int i = tid; i < kPrefixRows * CH; i += kThreads) {
+    const int r = i / CH, c = i % CH;
+    const bool ok = m0 + r < queries;
+    const long long m = ok ? m0 + r : m0;
+    const long long b = m / p.per;
+    const int h = kvh * p.per + (int)(m % p.per);
+    cp_async16(sm + tile_at<D>(r, c), q + b * p.q_row + h * p.q_head + c * 8, ok);
+  }
+  const int g0 = max(0, row_group(p, (int)(m0 / p.per)));
+  near_starts[tid] = p.groups > 0 ? p.group_start[min(g0 + tid, p.groups)] : 0;
+  __syncthreads();
+  if (tid < kPrefixRows) {
+    const long long m = m0 + tid;
+    int b = -1, s = 0, len = 0, group = -1, begin = 0;
+    if (m < queries) {
+      b = (int)(m / p.per);
+      len = row_length(p, b, &s);
+      if (s < 0 || s >= p.g.slots) {
+        atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);
+        s = 0;
+      }
+      if (p.groups > 0) {
+        const int k = last_not_above(near_starts, kThreads, b);
+        if (k + 1 < kThreads && near_starts[k] <= b && near_starts[k + 1] > b && g0 + k < p.groups)
+          group = g0 + k;
+        else if (p.group_start[0] <= b && p.group_start[p.groups] > b)  // behind the starts at hand
+          group = last_not_above(p.group_start, p.groups, b);
+      }
+      begin = group_tokens(p, group);
+    }
+    row_of[tid] = b;
+    seq_of[tid] = s;
+    len_of[tid] = len;
+    begin_of[tid] = begin;
+    group_of[tid] = group;
+  }
+  __syncthreads();
+
+  const int wr = warp * 16, ra = wr + (lane >> 2), rb = ra + 8;
+  uint32_t qa[KS][4];
+  float o[NT][4];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  Running run;
+  // one step of this warp's 16 queries with the 16 keys at rows `row` of a tile; query x
+  // of the tile sees keys below lim[x]
+  auto step = [&](const uint8_t* sk, const uint8_t* sv, int row, int key0, int lim_a, int lim_b) {
+    float x[2][4] = {};
+    scores<T, D>(sk, row, qa, x);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int key = key0 + t * 8 + (lane & 3) * 2 + (e & 1);
+        x[t][e] = key < (e < 2 ? lim_a : lim_b) ? x[t][e] * p.scale_log2 : -INFINITY;
+      }
+    float fa, fb;
+    uint32_t pa[4];
+    softmax_step<T>(x, run, fa, fb, pa);
+    add_values<T, D>(sv, row, pa, fa, fb, o);
+  };
+
+  // ---- prefixes: the groups of the tile's rows in turn
+  bool have_q = false;
+  for (int x = 0; x < kPrefixRows;) {
+    const int group = group_of[x];
+    const int tokens = begin_of[x];
+    if (row_of[x] < 0) break;
+    // the rows of the group are consecutive
+    int after = x;
+#pragma unroll
+    for (int i = 0; i < kPrefixRows; i += 32)
+      after += __popc(__ballot_sync(0xffffffffu, i + lane >= x && group_of[i + lane] == group && row_of[i + lane] >= 0));
+    if (tokens == 0) {
+      x = after;
+      continue;
+    }
+    // read through the longest of the group's sequences (the first of them)
+    const int b0 = max(0, p.group_start[group]), b1 = min(p.rows, p.group_start[group + 1]);
+    int len = -1, row = b1;
+    for (int b = b0 + tid; b < b1; b += kThreads) {
+      int s;
+      const int t = row_length(p, b, &s);
+      if (t > len) {
+        len = t;
+        row = b;
+      }
+    }
+#pragma unroll
+    for (int w = 16; w; w >>= 1) {
+      const int l2 = __shfl_xor_sync(0xffffffffu, len, w), r2 = __shfl_xor_sync(0xffffffffu, row, w);
+      if (l2 > len || (l2 == len && r2 < row)) {
+        len = l2;
+        row = r2;
+      }
+    }
+    if (lane == 0) {
+      lead_len[warp] = len;
+      lead_row[warp] = row;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 4; ++w)
+      if (lead_len[w] > len || (lead_len[w] == len && lead_row[w] < row)) {
+        len = lead_len[w];
+        row = lead_row[w];
+      }
+    const int common = max(0, min(tokens, len));
+    const int* lead = p.table + (long long)(len > 0 ? p.seqs[row] : 0) * p.g.width;
+    const int units = (common + kUnit - 1) / kUnit, steps = (units + 3) / 4;
+    auto load = [&](int j) {
+      uint8_t* kd = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+      const int keys = min(4, units - j * 4) * kUnit;
+      for (int i = tid; i < keys * CH; i += kThreads) {
+        const int r = i / CH, c = i % CH;
+        const int t = (j * 4 + r / kUnit) * kUnit;
+        const int page = lead[t / P];
+        const bool ok = page_ok(page, p.g.pages);
+        const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P + r % kUnit) * CH + c;
+        cp_async16(kd + tile_at<D>(r, c), pool + at, ok);
+        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + to_v, ok);
+        if (c == 0 && r % kUnit == 0) {
+          unit_ok[j & 1][r / kUnit] = ok;
+          if (!ok) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+        }
+      }
+      cp_async_commit();
+    };
+    if (steps > 0) load(0);
+    const int lim_a = ra >= x && ra < after ? min(common, len_of[ra]) : 0;
+    const int lim_b = rb >= x && rb < after ? min(common, len_of[rb]) : 0;
+    for (int j = 0; j < steps; ++j) {
+      if (j + 1 < steps) {
+        load(j + 1);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      __syncthreads();
+      if (!have_q) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
+        have_q = true;
+      }
+      const uint8_t* sk = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+      if (__any_sync(0xffffffffu, lim_a > 0 || lim_b > 0))
+        for (int h = 0; h < min(4, units - j * 4); ++h)
+          if (unit_ok[j & 1][h]) step(sk, sk + TILE, h * kUnit, (j * 4 + h) * kUnit, lim_a, lim_b);
+      __syncthreads();
+    }
+    __syncthreads();  // lead_len is free again
+    x = after;
+  }
+  cp_async_wait_all();
+  __syncthreads();  // Q is there, and the prefix tiles are free
+  if (!have_q) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
+  }
+
+  // ---- own keys: this warp's rows in turn, (first query x, unit u)
+  uint8_t* ring = sm + kPrefixRows * D * 2 + warp * 4 * UNIT;
+  auto units_of = [&](int x) {
+    const int own = len_of[x] - begin_of[x];
+    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
+  };
+  auto next_row = [&](int x) {  // the first query of the next row
+    const int b = row_of[x];
+    do ++x;
+    while (x < wr + 16 && row_of[x] == b);
+    return x;
+  };
+  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 16: none
+    while (x < wr + 16 && (row_of[x] < 0 || u >= units_of(x))) {
+      x = row_of[x] < 0 ? wr + 16 : next_row(x);
+      u = 0;
+    }
+  };
+  unsigned ok_bits = 0;
+  auto load = [&](int x, int u, int n) {
+    uint8_t* kd = ring + (n & 1) * 2 * UNIT;
+    const int t = begin_of[x] + u * kUnit, len = len_of[x];
+    const int page = p.table[(long long)seq_of[x] * p.g.width + t / P];
+    const bool ok = page_ok(page, p.g.pages);
+    ok_bits = (ok_bits & ~(1u << (n & 1))) | ((unsigned)ok << (n & 1));
+    if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+    const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P) * CH;
+#pragma unroll
+    for (int i = 0; i < kUnit * CH / 32; ++i) {
+      const int y = i * 32 + lane, r = y / CH, c = y % CH;
+      const bool in = ok && t + r < len;  // rows behind the sequence hold anything: zero instead
+      cp_async16(kd + tile_at<D>(r, c), pool + at + y, in);
+      cp_async16(kd + UNIT + tile_at<D>(r, c), pool + at + to_v + y, in);
+    }
+    cp_async_commit();
+  };
+  int x = wr, u = 0;
+  skip(x, u);
+  if (x < wr + 16) load(x, u, 0);
+  for (int n = 0; x < wr + 16; ++n) {
+    int nx = x, nu = u + 1;
+    skip(nx, nu);
+    if (nx < wr + 16) {
+      load(nx, nu, n + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncwarp();
+    if (ok_bits >> (n & 1) & 1) {
+      const uint8_t* sk = ring + (n & 1) * 2 * UNIT;
+      const int b = row_of[x], len = len_of[x];
+      step(sk, sk + UNIT, 0, begin_of[x] + u * kUnit, row_of[ra] == b ? len : 0, row_of[rb] == b ? len : 0);
+    }
+    __syncwarp();  // the stage may be loaded again
+    x = nx;
+    u = nu;
+  }
+  join_lanes(run);
+
+  // ---- result, through this warp's own rows of Q
+  const float ia = len_of[ra] > 0 ? 1.f / run.la : 0.f, ib = len_of[rb] > 0 ? 1.f / run.lb : 0.f;
+  bool ok_a = len_of[ra] == 0 || (run.la > 0.f && finite_f(run.la));
+  bool ok_b = len_of[rb] == 0 || (run.lb > 0.f && finite_f(run.lb));
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    ok_a = ok_a && finite_f(o[t][0]) && finite_f(o[t][1]);
+    ok_b = ok_b && finite_f(o[t][2]) && finite_f(o[t][3]);
+    const int c = t ^ (ra & 7);  // ra and rb have the same low bits
+    uint8_t* at = sm + ra * (D * 2) + (c << 4) + (lane & 3) * 4;
+    *reinterpret_cast<uint32_t*>(at) = Elem<T>::pack(o[t][0] * ia, o[t][1] * ia);
+    *reinterpret_cast<uint32_t*>(at + 8 * D * 2) = Elem<T>::pack(o[t][2] * ib, o[t][3] * ib);
+  }
+  const unsigned bad_a = __ballot_sync(0xffffffffu, !ok_a), bad_b = __ballot_sync(0xffffffffu, !ok_b);
+  __syncwarp();
+#pragma unroll
+  for (int i = lane; i < 16 * CH; i += 32) {
+    const int r = wr + i / CH, c = i % CH, b = row_of[r];
+    if (b < 0) continue;
+    const int h = kvh * p.per + (int)((m0 + r) % p.per);
+    *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + b * p.o_row + h * p.o_head + c * 8) =
+        *reinterpret_cast<const uint4*>(sm + tile_at<D>(r, c));
+  }
+  if ((bad_a | bad_b) == 0) return;
+  __syncwarp();
+  for (int r = 0; r < 16; ++r)
+    if (((r < 8 ? bad_a : bad_b) >> ((r & 7) * 4) & 0xf) && row_of[wr + r] >= 0)
+      row_again<T, D>(p, row_of[wr + r], kvh * p.per + (int)((m0 + wr + r) % p.per));
+}
+
 // Joins the ranges of each (row, head): a warp each, D / 32 dims per lane.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
@@ -557,10 +835,16 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   long long n = (8LL * sms + items - 1) / items;
   if (n > own / 64) n = own / 64;
   p->own_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+  // One pass where its blocks fill the GPU and a warp has at most 64 steps of own keys
+  // for its 16 queries and 16 of a prefix, one behind the other.
+  const long long blocks = ((long long)a->rows * p->per + kPrefixRows - 1) / kPrefixRows * K;
+  const long long rows = (16 + p->per - 1) / p->per, steps = rows * ((own + kUnit - 1) / kUnit);
+  p->whole = blocks >= 2LL * sms && steps <= 64 &&
+             (!prefix || (long long)a->prefix_pages_hint * a->cache->page_size <= 16 * kPrefixKeys);
 }
 
 size_t partial_bytes(const OasisSharedArgs* a, const SharedParams& p) {
-  if (p.prefix_splits == 0 && p.own_splits == 1) return 0;
+  if (p.whole || (p.prefix_splits == 0 && p.own_splits == 1)) return 0;
   const size_t slots = (size_t)a->rows * a->heads * (p.prefix_splits + p.own_splits);
   return slots * (sizeof(float2) + sizeof(float) * a->cache->head_dim);
 }
@@ -574,9 +858,16 @@ int launch(const SharedParams& p, cudaStream_t s) {
     cudaError_t e =
         cudaFuncSetAttribute(shared_prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<D>());
     if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(shared_whole_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<D>());
+    if (e == cudaSuccess)
       e = cudaFuncSetAttribute(shared_own_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem<D>());
     if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     attr[dev & 63] = true;
+  }
+  if (p.whole) {
+    const long long blocks = ((long long)p.rows * p.per + kPrefixRows - 1) / kPrefixRows * p.g.kv_heads;
+    launch_pdl(shared_whole_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
+    return check_launch("shared_whole_kernel");
   }
   if (p.prefix_splits) {
     const long long blocks = (long long)p.groups * p.g.kv_heads * p.prefix_splits * p.tiles;
@@ -646,6 +937,7 @@ int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream) {
                   "attention_shared: stride %lld is not a positive multiple of 8 elements", s);
   SharedParams p;
   plan(a, &p);
+  p.groups = a->groups > 0 && a->prefix_pages_hint > 0 ? a->groups : 0;
   const long long blocks = (long long)a->groups * c->kv_heads * (p.prefix_splits ? p.prefix_splits : 1) * p.tiles;
   const long long items = (long long)a->rows * c->kv_heads * p.head_tiles * p.own_splits;
   OASIS_REQUIRE(blocks < (1LL << 31) && items < (1LL << 31), "attention_shared: %d rows of %d heads are too many",
@@ -679,7 +971,6 @@ int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream) {
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (size_t)a->rows * a->heads * (p.prefix_splits + p.own_splits) *
                                                        c->head_dim);
   p.rows = a->rows;
-  p.groups = a->groups;
   p.heads = a->heads;
   p.layer = a->layer;
   p.scale_log2 = a->scale * kLog2e;
