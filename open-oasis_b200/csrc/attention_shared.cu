@@ -25,7 +25,8 @@ constexpr int kPrefixRows = 64;     // (row, head) queries of a block
 constexpr int kPrefixKeys = 64;     // keys of a step
 constexpr int kThreads = 128;
 constexpr int kOwnWarps = 4;
-constexpr int kMostSplits = 64;
+constexpr int kMostSplits = 64;    // of a prefix, and of a row's own keys
+constexpr int kMostRanges = 2 * kMostSplits;
 
 struct SharedParams {
   PageGeometry g;
@@ -37,7 +38,7 @@ struct SharedParams {
   float* part_o;   // [rows heads][splits][D]
   float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
   int rows, groups, heads, per, layer;  // per: heads of a key head
-  int prefix_splits, own_splits, tiles, head_tiles, whole;
+  int prefix_splits, own_splits, own_units, tiles, head_tiles, whole;  // own_units: of a split but the last
   float scale_log2;
 };
 
@@ -365,7 +366,8 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   const int group = p.prefix_splits ? row_group(p, b) : -1;
   const int begin = group_tokens(p, group);
   const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
-  const int u0 = (int)((long long)units * split / p.own_splits), u1 = (int)((long long)units * (split + 1) / p.own_splits);
+  const int u0 = min(units, split * p.own_units), u1 = split + 1 < p.own_splits ? min(units, u0 + p.own_units) : units;
+  if (split > 0 && u0 == units) return;  // a shorter row has fewer ranges
   const int* table = p.table + (long long)s * p.g.width;
   const uint4* pool = static_cast<const uint4*>(p.pool);
   const int nh = min(16, p.per - ht * 16), h0 = kvh * p.per + ht * 16;  // heads of this fragment
@@ -786,18 +788,60 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
   const int first = p.prefix_splits && row_group(p, b) >= 0 ? 0 : p.prefix_splits;
   int s;
   const int len = row_length(p, b, &s);
-  float m = -INFINITY, l = 0.f, o[DV] = {};
-  for (int i = first; i < splits; ++i) {
-    const float2 ml = p.part_ml[item * splits + i];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float n = fmaxf(m, ml.x), sh = softmax_shift(n);
-    const float fo = ex2_approx(m - sh), fp = ex2_approx(ml.x - sh);
-    l = l * fo + ml.y * fp;
-    m = n;
-    const float* y = p.part_o + (item * splits + i) * D + lane * DV;
+  // the row's ranges: the prefix ones and as many own ones as its length has
+  const int begin = first == 0 ? group_tokens(p, row_group(p, b)) : 0;
+  const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
+  const int last = p.prefix_splits + min(p.own_splits, max(1, (units + p.own_units - 1) / p.own_units));
+  const float2* ml = p.part_ml + item * splits;
+  // all maxima and sums at once, four ranges per lane
+  float2 mine[kMostRanges / 32];
+  float m = -INFINITY;
 #pragma unroll
-    for (int d = 0; d < DV; ++d) o[d] = o[d] * fo + y[d] * fp;
+  for (int k = 0; k < kMostRanges / 32; ++k) {
+    const int i = first + k * 32 + lane;
+    mine[k] = i < last ? ml[i] : make_float2(-INFINITY, 0.f);
+    m = fmaxf(m, mine[k].x);
   }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
+  const float sh = softmax_shift(m);
+  float l = 0.f, o[DV] = {};
+#pragma unroll
+  for (int k = 0; k < kMostRanges / 32; ++k) {
+    const float f = ex2_approx(mine[k].x - sh);
+    l += mine[k].y * f;
+    const bool some = !(mine[k].x == -INFINITY && mine[k].y == 0.f);  // its sums were written
+    unsigned todo = __ballot_sync(0xffffffffu, some);
+    while (todo) {  // four ranges' loads in flight
+      float4 y[4];
+      float g[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = todo ? __ffs(todo) - 1 : -1;
+        todo &= todo - 1;
+        g[e] = i >= 0 ? __shfl_sync(0xffffffffu, f, i) : 0.f;
+        y[e] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (i >= 0) {
+          const float* at = p.part_o + (item * splits + first + k * 32 + i) * D + lane * DV;
+          if constexpr (DV == 4) {
+            y[e] = *reinterpret_cast<const float4*>(at);
+          } else {
+            const float2 z = *reinterpret_cast<const float2*>(at);
+            y[e].x = z.x;
+            y[e].y = z.y;
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float v[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
+#pragma unroll
+        for (int d = 0; d < DV; ++d) o[d] = fmaf(v[d], g[e], o[d]);
+      }
+    }
+  }
+#pragma unroll
+  for (int w = 16; w; w >>= 1) l += __shfl_xor_sync(0xffffffffu, l, w);
   bool ok = len == 0 || (l > 0.f && finite_f(l));
 #pragma unroll
   for (int d = 0; d < DV; ++d) ok = ok && finite_f(o[d]);
@@ -829,12 +873,18 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
     if (n > keys / 128) n = keys / 128;
     p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
   }
-  // eight warps for each SM, and at least 64 keys for each warp
+  // A row's own keys go to warps in ranges of one length, so that a row longer than the
+  // others only has more of them: at least 128 keys, as many ranges as make 48 warps for
+  // each SM where all rows have the hinted length.
   const long long items = (long long)a->rows * K * p->head_tiles;
   const long long own = a->own_tokens_hint;
-  long long n = (8LL * sms + items - 1) / items;
-  if (n > own / 64) n = own / 64;
-  p->own_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+  long long n = (48LL * sms + items - 1) / items;
+  if (n > kMostSplits) n = kMostSplits;
+  const long long units = (own + kUnit - 1) / kUnit;
+  long long each = (units + n - 1) / n;
+  if (each < 8) each = 8;
+  p->own_units = (int)each;
+  p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
   // One pass where its blocks fill the GPU and a warp has at most 64 steps of own keys
   // for its 16 queries and 16 of a prefix, one behind the other.
   const long long blocks = ((long long)a->rows * p->per + kPrefixRows - 1) / kPrefixRows * K;
