@@ -18,7 +18,7 @@ LIB_NAME = "liboasis_b200.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 SOURCES = ["gemm.cu", "attention.cu", "attention_tc.cu", "pointwise.cu", "capi.cu", "static_scratch.cu", "cond.cu", "peer.cu",
            "pages.cu", "attention_prompt.cu", "attention_prompt_tc.cu",
-           "attention_shared.cu"]
+           "attention_shared.cu", "attention_shared_tc.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

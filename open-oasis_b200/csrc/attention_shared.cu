@@ -13,63 +13,24 @@
 // writes the result; otherwise shared_join_kernel does.
 #include "../../include/oasis_b200.h"
 #include "attention_rows.cuh"
+#include "attention_shared.cuh"
 #include "gemm.cuh"
-#include "pages.cuh"
 #include "status.h"
 
 namespace oasis {
 namespace {
 
-constexpr int kUnit = 16;           // keys of a step of a warp: always inside one page
 constexpr int kPrefixRows = 64;     // (row, head) queries of a block
 constexpr int kPrefixKeys = 64;     // keys of a step
 constexpr int kThreads = 128;
 constexpr int kOwnWarps = 4;
+// Prefixes of at least this many tokens run on the tensor-memory kernel.
+#ifndef OASIS_TENSOR_KEYS
+#define OASIS_TENSOR_KEYS 256
+#endif
+constexpr int kTensorKeys = OASIS_TENSOR_KEYS;
 constexpr int kMostSplits = 64;    // of a prefix, and of a row's own keys
 constexpr int kMostRanges = 2 * kMostSplits;
-
-struct SharedParams {
-  PageGeometry g;
-  const void *q, *pool;
-  void* out;
-  long long q_row, q_head, o_row, o_head;
-  const int *table, *lengths, *seqs, *group_start, *prefix_pages;
-  int* status;
-  float* part_o;   // [rows heads][splits][D]
-  float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
-  int rows, groups, heads, per, layer;  // per: heads of a key head
-  int prefix_splits, own_splits, own_units, tiles, head_tiles, whole;  // own_units: of a split but the last
-  float scale_log2;
-};
-
-// Length of row b's sequence, 0 where there is none; `s` its slot.
-__device__ __forceinline__ int row_length(const SharedParams& p, int b, int* s) {
-  const int x = p.seqs[b];
-  *s = x;
-  if (x < 0 || x >= p.g.slots) return 0;
-  return held_tokens(p.lengths[x], p.g.page_size, p.g.width);
-}
-
-// Group of row b, by the whole warp: the last one that starts at or before b; -1
-// where b lies outside of them.
-__device__ __forceinline__ int row_group(const SharedParams& p, int b) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = p.groups;  // the answer is in [lo, lo + n)
-  if (n < 1 || p.group_start[0] > b || p.group_start[p.groups] <= b) return -1;
-  while (n > 1) {
-    const int step = (n + 31) / 32;
-    const int i = lane * step;
-    const bool ok = i < n && p.group_start[lo + i] <= b;
-    const int c = 32 - __clz(__ballot_sync(0xffffffffu, ok) | 1u);  // probes that hold: a run from lane 0
-    lo += (c - 1) * step;
-    n = min(step, n - (c - 1) * step);
-  }
-  return lo;
-}
-
-__device__ __forceinline__ int group_tokens(const SharedParams& p, int group) {
-  return group < 0 ? 0 : held_tokens(p.prefix_pages[group], 1, p.g.width) * p.g.page_size;
-}
 
 template <int D>
 constexpr int prefix_smem() {
@@ -363,7 +324,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     if (lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);
     s = 0;
   }
-  const int group = p.prefix_splits ? row_group(p, b) : -1;
+  const int group = served_group(p, b);
   const int begin = group_tokens(p, group);
   const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
   const int u0 = min(units, split * p.own_units), u1 = split + 1 < p.own_splits ? min(units, u0 + p.own_units) : units;
@@ -785,11 +746,11 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
   if (item >= (long long)p.rows * p.heads) return;
   const int b = (int)(item / p.heads), h = (int)(item - (long long)b * p.heads);
   const int splits = p.prefix_splits + p.own_splits;
-  const int first = p.prefix_splits && row_group(p, b) >= 0 ? 0 : p.prefix_splits;
+  const int group = served_group(p, b), first = group >= 0 ? 0 : p.prefix_splits;
   int s;
   const int len = row_length(p, b, &s);
   // the row's ranges: the prefix ones and as many own ones as its length has
-  const int begin = first == 0 ? group_tokens(p, row_group(p, b)) : 0;
+  const int begin = group_tokens(p, group);
   const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
   const int last = p.prefix_splits + min(p.own_splits, max(1, (units + p.own_units - 1) / p.own_units));
   const float2* ml = p.part_ml + item * splits;
@@ -865,13 +826,28 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
   p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);
   p->prefix_splits = 0;
+  p->tensor = 0;
+  p->reach = 0x7fffffff;
   if (prefix) {
-    // two blocks for each SM, and at least 128 keys for each block
-    const long long blocks = (long long)a->groups * K * p->tiles;
     const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
-    long long n = (2LL * sms + blocks - 1) / blocks;
-    if (n > keys / 128) n = keys / 128;
-    p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
+    p->tensor = keys >= kTensorKeys && pool_rows < (1LL << 31);
+    if (p->tensor) {
+      // one block for each SM, and at least 128 keys for each block
+      const long long pairs = ((long long)group_rows * p->per + 255) / 256;
+      p->tiles = (int)pairs;
+      p->reach = pairs * 256 < 0x7fffffff ? (int)pairs * 256 : 0x7fffffff;
+      const long long blocks = (long long)a->groups * K * pairs;
+      long long n = sms / blocks;
+      if (n > keys / 128) n = keys / 128;
+      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    } else {
+      // two blocks for each SM, and at least 128 keys for each block
+      const long long blocks = (long long)a->groups * K * p->tiles;
+      long long n = (2LL * sms + blocks - 1) / blocks;
+      if (n > keys / 128) n = keys / 128;
+      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    }
   }
   // A row's own keys go to warps in ranges of one length, so that a row longer than the
   // others only has more of them: at least 128 keys, as many ranges as make 48 warps for
@@ -919,7 +895,9 @@ int launch(const SharedParams& p, cudaStream_t s) {
     launch_pdl(shared_whole_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
     return check_launch("shared_whole_kernel");
   }
-  if (p.prefix_splits) {
+  if (p.prefix_splits && p.tensor) {
+    OASIS_TRY(shared_prefix_tc_launch(p, Elem<T>::kHalf, s));
+  } else if (p.prefix_splits) {
     const long long blocks = (long long)p.groups * p.g.kv_heads * p.prefix_splits * p.tiles;
     launch_pdl(shared_prefix_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
     OASIS_TRY(check_launch("shared_prefix_kernel"));

@@ -32,6 +32,7 @@ int set_error(int code, const char* fmt, ...) {
 int read_device_error(int reset);  // gemm.cu
 int read_device_error_peer(int reset);  // peer.cu
 int read_device_error_prompt(int reset);  // attention_prompt_tc.cu
+int read_device_error_shared(int reset);  // attention_shared_tc.cu
 
 bool pdl_enabled() {
   static const bool on = [] {
@@ -1114,7 +1115,8 @@ int oasis_device_error(int reset) {
   const int b = read_device_error_tc(reset);
   const int c = read_device_error_peer(reset);
   const int d = read_device_error_prompt(reset);
-  return a ? a : (b ? b : (c ? c : d));
+  const int e = read_device_error_shared(reset);
+  return a ? a : (b ? b : (c ? c : (d ? d : e)));
 }
 
 unsigned long long oasis_launch_count(void) { return g_launches.load(std::memory_order_relaxed); }

@@ -188,6 +188,24 @@ def test_what_is_not_seen_takes_no_part(hint, bad, dim):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_a_score_that_is_not_finite_reaches_the_result(hint, dtype, bad):
+    """One key of NaN, or one that scores +inf, at each place of a block in turn, its value
+    finite: every row that sees it is NaN, no other is."""
+    n = 130
+    q, k, v = inputs([n], 1, 1, 64, dtype, seed=13)
+    q[:, :, 0] = 1
+    for at in list(range(0, n, 7)) + [126, 127, 128, 129]:
+        kk = k.clone()
+        kk[at, 0, 0] = bad
+        got = paged.attention_prompt(q, kk, v, ints([0, n]), hint)
+        seen = torch.isnan(got).reshape(n, -1)
+        assert bool(seen[at:].all()) and not bool(seen[:at].any()), at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
 def test_keys_at_the_lowest_value(hint):
     """Scores of -inf and of the type's lowest value before, between and after others."""
     lengths = [260]

@@ -138,6 +138,8 @@ def test_plan_is_checked():
 # --------------------------------------------------------------------- on a GPU --
 
 GROUPS = {
+    "long prefix": [(33, [600, 540, 528]), (80, [1290, 1281])],
+    "long and short": [(40, [645, 100, 0, 700, 639, 641]), (2, [33])],
     "one row": [(0, [1])],
     "lengths": [(0, [1, 15, 16, 17, 0, 64, 65, 200])],
     "prefix": [(2, [33, 40, 32, 64])],
@@ -165,6 +167,85 @@ def test_groups(name, heads, kv, dim, dtype, page):
     alone = paged.SharedPlan([], [], plan.longest, DEV)
     check(paged.attention_shared(q, c, 1, ints(seqs), alone), q, c, 1, seqs)
     c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv,dim,dtype,page", [(32, 16, 64, BF16, 16), (20, 20, 128, FP16, 32), (112, 16, 64, FP16, 48)])
+@pytest.mark.parametrize("shape", ["forks", "ragged", "alone"])
+def test_many_rows_with_few_keys(shape, heads, kv, dim, dtype, page):
+    """Enough rows for the one-pass kernel: groups inside, across and larger than a tile,
+    short and empty rows, rows in no group."""
+    rng = random.Random(7)
+    n = 64 * 20 * kv // heads
+    if shape == "forks":
+        groups = [(1, [page + rng.randint(1, page) for _ in range(16)]) for _ in range(n // 16)]
+    elif shape == "ragged":
+        groups, left = [], n
+        while left > 0:
+            r = min(left, rng.choice([1, 2, 5, 150]))
+            p = rng.choice([0, 1, 3])
+            groups.append((p, [rng.choice([0, 3, p * page, p * page + rng.randint(1, 40)]) for _ in range(r)]))
+            left -= r
+    else:
+        groups = [(0, [rng.randint(0, 50) for _ in range(n)])]
+    c, seqs, plan, g = build(groups, page, kv, dim, dtype, layers=1)
+    if shape == "ragged":  # the last rows belong to no group
+        plan.group_start[-1] -= 1
+    q = queries(len(seqs), heads, dim, dtype, g)
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    check(got, q, c, 0, seqs)
+    assert torch.equal(got, paged.attention_shared(q, c, 0, ints(seqs), plan))
+    c.pool[:, :, 1, :, -1] = math.nan  # values behind many rows' last token, seen by others
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    want = O.attention_cached(q, c.pool, c.table.tolist(), c.lengths.tolist(), 0, seqs)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and bool(torch.isnan(want).any())
+    fine = ~torch.isnan(want).reshape(len(seqs), -1).any(1)
+    c.pool[:, :, 1] = torch.nan_to_num(c.pool[:, :, 1])
+    check(got, q, c, 0, seqs, rows=fine)
+    c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,heads,kv,dim,dtype,page", [
+    (300, 2, 2, 64, BF16, 16), (70, 12, 3, 128, BF16, 64), (40, 7, 1, 64, FP16, 48), (140, 2, 1, 128, FP16, 128), (3, 4, 4, 64, BF16, 256),
+])
+def test_long_prefixes(rows, heads, kv, dim, dtype, page):
+    """The tensor-memory kernel: both tiles, several ranges, pages above and below a block,
+    rows of different limits, a page of the prefix that is not in the pool, hints that are
+    too small."""
+    rng = random.Random(rows)
+    first = -(-900 // page)
+    groups = [(first, [first * page + rng.choice([-200, 0, 1, 33]) for _ in range(rows - 1)] + [first * page + 5]),
+              (-(-300 // page), [-(-300 // page) * page + 2] * 2)]
+    c, seqs, plan, g = build(groups, page, kv, dim, dtype)
+    q = queries(len(seqs), heads, dim, dtype, g)
+    good = paged.attention_shared(q, c, 1, ints(seqs), plan)
+    check(good, q, c, 1, seqs)
+    assert torch.equal(good, paged.attention_shared(q, c, 1, ints(seqs), plan))
+    plan.most_rows, pages = 1, plan.most_pages
+    check(paged.attention_shared(q, c, 1, ints(seqs), plan), q, c, 1, seqs)
+    plan.most_rows, plan.most_pages = rows, 10 * pages
+    check(paged.attention_shared(q, c, 1, ints(seqs), plan), q, c, 1, seqs)
+    plan.most_pages = pages
+    shared = int(c.table[seqs[0], 1])
+    c.pool[shared, 1, 0, 0, 3, :] = math.nan  # a key of the prefix
+    got = paged.attention_shared(q, c, 1, ints(seqs), plan)
+    want = O.attention_cached(q, c.pool, c.table.tolist(), c.lengths.tolist(), 1, seqs)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and bool(torch.isnan(want).any())
+    c.pool[shared, 1, 0, 0, 3, :] = 0
+    c.check()
+    c.table[torch.tensor(seqs[:rows], device=DEV), 1] = -7  # left out of the sum, for all rows alike
+    got = paged.attention_shared(q, c, 1, ints(seqs), plan)
+    torch.cuda.synchronize()
+    assert int(c.status.item()) == paged.BAD_PAGE
+    table, lengths = c.table.tolist(), c.lengths.tolist()
+    for b in (0, rows - 1):
+        s = seqs[b]
+        pages = [p for i, p in enumerate(table[s][: -(-lengths[s] // page)]) if i != 1]
+        kv_rows = c.pool[pages, 1].permute(1, 2, 0, 3, 4).reshape(2, kv, -1, dim)[:, :, : lengths[s] - page]
+        want = O.attention_rows(q[b : b + 1], kv_rows[0].transpose(0, 1), kv_rows[1].transpose(0, 1))
+        assert float((got[b].double() - want[0]).norm() / want.norm()) < 2 * torch.finfo(dtype).eps
+    assert _lib.load().oasis_device_error(0) == 0
 
 
 @pytest.mark.gpu
