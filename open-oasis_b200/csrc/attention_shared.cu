@@ -7,9 +7,9 @@
 //
 // shared_prefix_kernel: the keys that a group's rows have in common, read once for all
 // of them: 64 (row, head) queries of one key head per block, 64 keys a step, mma.sync.
-// shared_own_kernel: each row's keys behind the prefix: a warp per (row, key head,
-// split), 16 keys a step, the heads of a group as the 16 rows of a fragment. Bound by
-// reading the keys and values once. With one split it joins the prefix ranges too and
+// shared_own_kernel: each row's keys behind the prefix: four warps (or one) per (row, key
+// head, range), 16 keys a step, the heads of a key head as the 16 rows of a fragment.
+// Bound by reading the keys and values once. With one split it joins the prefix ranges too and
 // writes the result; otherwise shared_join_kernel does.
 #include "../../include/oasis_b200.h"
 #include "attention_rows.cuh"
@@ -125,8 +125,8 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
   __shared__ int limit[kPrefixRows];  // keys that a query sees; -1: no query
   __shared__ int lead_len[4], lead_row[4];
   __shared__ int unit_ok[2][4];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // behind the wait: the kernel of the own keys starts without one
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int x = blockIdx.x;
   const int tile = x % p.tiles;
@@ -305,19 +305,25 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams p) {
   constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kUnit * D * 2;
   extern __shared__ __align__(128) uint8_t sm[];
+  // Behind a prefix kernel this one starts when every block of that one is past its own
+  // wait, so that all before it is done; its ranges are waited for where they are joined.
   pdl_trigger();
-  pdl_wait();
+  if (!p.prefix_splits) pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint8_t* ring = sm + warp * 4 * TILE;
-  const long long item = (long long)blockIdx.x * kOwnWarps + warp;
-  long long x = item;
+  // an item is a warp's, or a team of four warps takes its units in turn
+  const int member = p.team > 1 ? warp : 0;
+  long long x = p.team > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * kOwnWarps + warp;
   const int split = (int)(x % p.own_splits);
   x /= p.own_splits;
   const int ht = (int)(x % p.head_tiles);
   x /= p.head_tiles;
   const int kvh = (int)(x % p.g.kv_heads);
   const int b = (int)(x / p.g.kv_heads);
-  if (b >= p.rows) return;  // whole warps; no block-wide barrier follows
+  if (b >= p.rows) {  // whole warps, and whole teams
+    pdl_wait();
+    return;
+  }
   int s;
   const int len = row_length(p, b, &s), P = p.g.page_size;
   if (s < 0 || s >= p.g.slots) {
@@ -328,18 +334,21 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   const int begin = group_tokens(p, group);
   const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
   const int u0 = min(units, split * p.own_units), u1 = split + 1 < p.own_splits ? min(units, u0 + p.own_units) : units;
-  if (split > 0 && u0 == units) return;  // a shorter row has fewer ranges
+  if (split > 0 && u0 == units) {  // a shorter row has fewer ranges
+    pdl_wait();
+    return;
+  }
   const int* table = p.table + (long long)s * p.g.width;
   const uint4* pool = static_cast<const uint4*>(p.pool);
   const int nh = min(16, p.per - ht * 16), h0 = kvh * p.per + ht * 16;  // heads of this fragment
 
   unsigned ok_bits = 0;  // of the two units in flight
-  auto load = [&](int u) {
-    uint8_t* kd = ring + (u & 1) * 2 * TILE;
+  auto load = [&](int u, int n) {
+    uint8_t* kd = ring + (n & 1) * 2 * TILE;
     const int t = begin + u * kUnit;
     const int page = table[t / P];
     const bool ok = page_ok(page, p.g.pages);
-    ok_bits = (ok_bits & ~(1u << (u & 1))) | ((unsigned)ok << (u & 1));
+    ok_bits = (ok_bits & ~(1u << (n & 1))) | ((unsigned)ok << (n & 1));
     if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
     const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P) * CH;
     const long long to_v = p.g.kv_heads * tile_vectors(p.g);
@@ -352,7 +361,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     }
     cp_async_commit();
   };
-  if (u0 < u1) load(u0);
+  if (u0 + member < u1) load(u0 + member, 0);
 
   const int ra = lane >> 2;
   const T* q = static_cast<const T*>(p.q) + b * p.q_row + h0 * p.q_head;
@@ -368,16 +377,16 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
   Running run;
-  for (int u = u0; u < u1; ++u) {
-    if (u + 1 < u1) {
-      load(u + 1);
+  for (int u = u0 + member, n = 0; u < u1; u += p.team, ++n) {
+    if (u + p.team < u1) {
+      load(u + p.team, n + 1);
       cp_async_wait<1>();
     } else {
       cp_async_wait<0>();
     }
     __syncwarp();
-    if (ok_bits >> (u & 1) & 1) {
-      const uint8_t* sk = ring + (u & 1) * 2 * TILE;
+    if (ok_bits >> (n & 1) & 1) {
+      const uint8_t* sk = ring + (n & 1) * 2 * TILE;
       float sc[2][4] = {};
       scores<T, D>(sk, 0, qa, sc);
 #pragma unroll
@@ -396,6 +405,57 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   }
   join_lanes(run);
 
+  if (p.team > 1) {  // the team's sums, in fragment order, to its first warp
+    float* mine = reinterpret_cast<float*>(ring) + lane;
+    __shared__ float4 stats[kOwnWarps][32];
+    if (member > 0) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mine[(t * 4 + e) * 32] = o[t][e];
+      stats[member][lane] = make_float4(run.ma, run.mb, run.la, run.lb);
+    }
+    __syncthreads();
+    if (member > 0) {
+      pdl_wait();
+      return;
+    }
+    float ma = run.ma, mb = run.mb;
+#pragma unroll
+    for (int w = 1; w < kOwnWarps; ++w) {
+      ma = fmaxf(ma, stats[w][lane].x);
+      mb = fmaxf(mb, stats[w][lane].y);
+    }
+    const float sa = softmax_shift(ma), sb = softmax_shift(mb);
+    const float ka = ex2_approx(run.ma - sa), kb = ex2_approx(run.mb - sb);
+    run.la *= ka;
+    run.lb *= kb;
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      o[t][0] *= ka;
+      o[t][1] *= ka;
+      o[t][2] *= kb;
+      o[t][3] *= kb;
+    }
+#pragma unroll
+    for (int w = 1; w < kOwnWarps; ++w) {
+      const float4 st = stats[w][lane];
+      const float fa = ex2_approx(st.x - sa), fb = ex2_approx(st.y - sb);
+      run.la = fmaf(st.z, fa, run.la);
+      run.lb = fmaf(st.w, fb, run.lb);
+      const float* other = reinterpret_cast<const float*>(sm + w * 4 * TILE) + lane;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        o[t][0] = fmaf(other[(t * 4 + 0) * 32], fa, o[t][0]);
+        o[t][1] = fmaf(other[(t * 4 + 1) * 32], fa, o[t][1]);
+        o[t][2] = fmaf(other[(t * 4 + 2) * 32], fb, o[t][2]);
+        o[t][3] = fmaf(other[(t * 4 + 3) * 32], fb, o[t][3]);
+      }
+    }
+    run.ma = ma;
+    run.mb = mb;
+  }
+
   const int splits = p.prefix_splits + p.own_splits;
   if (p.own_splits > 1) {
 #pragma unroll
@@ -411,9 +471,11 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
         *reinterpret_cast<float2*>(p.part_o + slot * D + t * 8 + (lane & 3) * 2) =
             make_float2(o[t][2 * half], o[t][2 * half + 1]);
     }
+    pdl_wait();  // nobody ends before the prefix kernel does: what follows waits for this one alone
     return;
   }
   // the prefix ranges of these heads join here
+  pdl_wait();
   unsigned bad = 0;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
@@ -773,11 +835,11 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
     l += mine[k].y * f;
     const bool some = !(mine[k].x == -INFINITY && mine[k].y == 0.f);  // its sums were written
     unsigned todo = __ballot_sync(0xffffffffu, some);
-    while (todo) {  // four ranges' loads in flight
-      float4 y[4];
-      float g[4];
+    while (todo) {  // eight ranges' loads in flight
+      float4 y[8];
+      float g[8];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const int i = todo ? __ffs(todo) - 1 : -1;
         todo &= todo - 1;
         g[e] = i >= 0 ? __shfl_sync(0xffffffffu, f, i) : 0.f;
@@ -794,7 +856,7 @@ __global__ void __launch_bounds__(kThreads) shared_join_kernel(SharedParams p) {
         }
       }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
+      for (int e = 0; e < 8; ++e) {
         const float v[4] = {y[e].x, y[e].y, y[e].z, y[e].w};
 #pragma unroll
         for (int d = 0; d < DV; ++d) o[d] = fmaf(v[d], g[e], o[d]);
@@ -849,16 +911,18 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
       p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
     }
   }
-  // A row's own keys go to warps in ranges of one length, so that a row longer than the
-  // others only has more of them: at least 128 keys, as many ranges as make 48 warps for
-  // each SM where all rows have the hinted length.
+  // A row's own keys go to teams of four warps in ranges of one length, so that a row
+  // longer than the others only has more of them: at least 256 keys, as many ranges as
+  // make 12 teams for each SM where all rows have the hinted length. Up to 32 keys are
+  // one warp's.
   const long long items = (long long)a->rows * K * p->head_tiles;
   const long long own = a->own_tokens_hint;
-  long long n = (48LL * sms + items - 1) / items;
+  long long n = (12LL * sms + items - 1) / items;
   if (n > kMostSplits) n = kMostSplits;
   const long long units = (own + kUnit - 1) / kUnit;
   long long each = (units + n - 1) / n;
-  if (each < 8) each = 8;
+  if (each < 16) each = 16;
+  p->team = units > 2 ? kOwnWarps : 1;
   p->own_units = (int)each;
   p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
   // One pass where its blocks fill the GPU and a warp has at most 64 steps of own keys
@@ -902,8 +966,8 @@ int launch(const SharedParams& p, cudaStream_t s) {
     launch_pdl(shared_prefix_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
     OASIS_TRY(check_launch("shared_prefix_kernel"));
   }
-  const long long items = (long long)p.rows * p.g.kv_heads * p.head_tiles * p.own_splits;
-  launch_pdl(shared_own_kernel<T, D>, dim3((unsigned)((items + kOwnWarps - 1) / kOwnWarps)), dim3(kOwnWarps * 32),
+  const long long items = (long long)p.rows * p.g.kv_heads * p.head_tiles * p.own_splits, in_block = kOwnWarps / p.team;
+  launch_pdl(shared_own_kernel<T, D>, dim3((unsigned)((items + in_block - 1) / in_block)), dim3(kOwnWarps * 32),
              own_smem<D>(), s, p);
   OASIS_TRY(check_launch("shared_own_kernel"));
   if (p.own_splits > 1) {

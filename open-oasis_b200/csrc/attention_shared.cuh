@@ -19,6 +19,7 @@ struct SharedParams {
   float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
   int rows, groups, heads, per, layer;  // per: heads of a key head
   int prefix_splits, own_splits, own_units, tiles, head_tiles, whole;  // own_units: of a split but the last
+  int team;    // warps of an item of own keys: 1 or 4
   int tensor;  // the prefix runs on the tensor-memory kernel
   int reach;   // (row, head) queries of a group and key head that the prefix kernel takes
   float scale_log2;

@@ -48,8 +48,8 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   using C = Cfg<D>;
   using E = Elem<T>;
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // behind the wait: the kernel of the own keys starts without one
   int x = blockIdx.x;
   const int pair = x % p.tiles;
   x /= p.tiles;
@@ -152,40 +152,54 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    if (warp == 8 && lane == 0) {
+    if (warp == 8) {
       // ---------------- TMA ----------------
-      const int total = 2 * blocks;
-      int issued = 0;
-      bool ok = true;
+      // A lane per box, with its page looked up one block ahead.
+      const int total = 2 * blocks, boxes = kTile / box_rows;
       const long long tile_rows = (long long)p.g.kv_heads * P;  // pool rows of a page's layer's keys, or values
-      for (; issued < total; ++issued) {
-        const int st = issued % C::STAGES;
-        if (issued >= C::STAGES && !wait_for(&kv_empty[st], ((issued / C::STAGES) & 1) ^ 1, kDevTimeoutSmemEmpty)) {
-          ok = false;
-          break;
-        }
-        uint8_t* dst = sKV + st * C::TILE_BYTES;
-        const int t0 = (begin + (issued >> 1)) * kTile, which = issued & 1;
-        int rows[kTile / kUnit];
+      auto page_at = [&](int block) {  // of this lane's box; -1: behind the prefix or not in the pool
+        const int t = block * kTile + lane * box_rows;
+        if (lane >= boxes || t >= common) return -1;
+        const int page = table[t / P];
+        if (page_ok(page, p.g.pages)) return page;
+        atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+        return -1;
+      };
+      int issued = 0, page = blocks > 0 ? page_at(begin) : -1;
+      bool ok = true;
+      while (issued < total && ok) {
+        const int block = begin + (issued >> 1);
+        const int ahead = (issued & 1) == 0 && issued + 2 < total ? page_at(block + 1) : -1;
+        const unsigned there = __ballot_sync(0xffffffffu, page >= 0);
         unsigned bits = 0;
-        for (int r = 0; r < kTile; r += box_rows) {
-          const int t = t0 + r;
-          const int page = t < common ? table[t / P] : -1;
-          const bool there = page_ok(page, p.g.pages);
-          if (there) bits |= ((1u << (box_rows / kUnit)) - 1) << (r / kUnit);
-          if (t < common && !there) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
-          rows[r / box_rows] =
-              there ? (int)((((long long)page * p.g.layers + p.layer) * 2 + which) * tile_rows + (long long)kvh * P + t % P) : pool_rows;
-        }
-        if (which == 0) {
-          page_bits[(issued >> 1) & 7] = bits;
-          __threadfence_block();
-        }
-        mbar_arrive_expect_tx(&kv_full[st], C::TILE_BYTES);
-        for (int r = 0; r < kTile; r += box_rows)
+        for (int i = 0; i < boxes; ++i)
+          if (there >> i & 1) bits |= ((1u << (box_rows / kUnit)) - 1) << (i * (box_rows / kUnit));
+        const int slot = (block * kTile + lane * box_rows) % P;
+        int next_page = ahead;
+        for (int which = 0; which < 2 && ok; ++which, ++issued) {
+          const int st = issued % C::STAGES;
+          if (issued >= C::STAGES)
+            ok = __all_sync(0xffffffffu, wait_for(&kv_empty[st], ((issued / C::STAGES) & 1) ^ 1, kDevTimeoutSmemEmpty));
+          if (!ok) break;
+          if (lane == 0) {
+            if (which == 0) {
+              page_bits[(issued >> 1) & 7] = bits;
+              __threadfence_block();
+            }
+            mbar_arrive_expect_tx(&kv_full[st], C::TILE_BYTES);
+          }
+          __syncwarp();  // the bytes are expected before they come
+          if (lane < boxes) {
+            uint8_t* dst = sKV + st * C::TILE_BYTES + lane * box_rows * 128;
+            const int row = page >= 0 ? (int)((((long long)page * p.g.layers + p.layer) * 2 + which) * tile_rows +
+                                              (long long)kvh * P + slot)
+                                      : pool_rows;
 #pragma unroll
-          for (int c = 0; c < C::CHUNKS; ++c)
-            tma_load_3d(dst + c * C::CHUNK_BYTES + r * 128, &pool_map, &kv_full[st], c * 64, rows[r / box_rows], 0);
+            for (int c = 0; c < C::CHUNKS; ++c)
+              tma_load_3d(dst + c * C::CHUNK_BYTES, &pool_map, &kv_full[st], c * 64, row, 0);
+          }
+        }
+        page = next_page;
       }
       if (!ok)  // gave up: the copies in flight land before the block ends
         for (int i = max(0, issued - C::STAGES); i < issued; ++i)
