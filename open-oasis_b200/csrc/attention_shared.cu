@@ -178,19 +178,18 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
 
   for (long long m0 = (long long)tile * kPrefixRows; m0 < queries; m0 += (long long)p.tiles * kPrefixRows) {
     __syncthreads();
+    const Queries at(m0, p.per);
     if (tid < kPrefixRows) {
-      const long long m = m0 + tid;
       int lim = -1, s;
-      if (m < queries) lim = min(common, row_length(p, b0 + (int)(m / p.per), &s));
+      if (m0 + tid < queries) lim = min(common, row_length(p, b0 + (int)at.row_of(tid), &s));
       limit[tid] = lim;
     }
     const T* q = static_cast<const T*>(p.q);
     for (int i = tid; i < kPrefixRows * CH; i += kThreads) {
       const int r = i / CH, c = i % CH;
       const bool ok = m0 + r < queries;
-      const long long m = ok ? m0 + r : m0;
-      const long long b = b0 + m / p.per;
-      const int h = kvh * p.per + (int)(m % p.per);
+      const long long b = b0 + at.row_of(ok ? r : 0);
+      const int h = kvh * p.per + at.head_of(ok ? r : 0);
       cp_async16(sm + tile_at<D>(r, c), q + b * p.q_row + h * p.q_head + c * 8, ok);
     }
     auto load = [&](int j) {
@@ -260,10 +259,9 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
     const int splits = p.prefix_splits + p.own_splits;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const long long m = m0 + ra + half * 8;
-      if (m >= queries) continue;
-      const long long b = b0 + m / p.per;
-      const int h = kvh * p.per + (int)(m % p.per);
+      if (m0 + ra + half * 8 >= queries) continue;
+      const long long b = b0 + at.row_of(ra + half * 8);
+      const int h = kvh * p.per + at.head_of(ra + half * 8);
       const long long slot = (b * p.heads + h) * splits + split;
       const float mm = half ? run.mb : run.ma, ll = half ? run.lb : run.la;
       if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm, ll);
@@ -543,6 +541,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.g.kv_heads;
   const long long m0 = (long long)(blockIdx.x / p.g.kv_heads) * kPrefixRows, queries = (long long)p.rows * p.per;
+  const Queries at_query(m0, p.per);
   const int P = p.g.page_size;
   const uint4* pool = static_cast<const uint4*>(p.pool);
   const long long to_v = p.g.kv_heads * tile_vectors(p.g);
@@ -550,19 +549,17 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   for (int i = tid; i < kPrefixRows * CH; i += kThreads) {
     const int r = i / CH, c = i % CH;
     const bool ok = m0 + r < queries;
-    const long long m = ok ? m0 + r : m0;
-    const long long b = m / p.per;
-    const int h = kvh * p.per + (int)(m % p.per);
+    const long long b = at_query.row_of(ok ? r : 0);
+    const int h = kvh * p.per + at_query.head_of(ok ? r : 0);
     cp_async16(sm + tile_at<D>(r, c), q + b * p.q_row + h * p.q_head + c * 8, ok);
   }
-  const int g0 = max(0, row_group(p, (int)(m0 / p.per)));
+  const int g0 = max(0, row_group(p, (int)at_query.row));
   near_starts[tid] = p.groups > 0 ? p.group_start[min(g0 + tid, p.groups)] : 0;
   __syncthreads();
   if (tid < kPrefixRows) {
-    const long long m = m0 + tid;
     int b = -1, s = 0, len = 0, group = -1, begin = 0;
-    if (m < queries) {
-      b = (int)(m / p.per);
+    if (m0 + tid < queries) {
+      b = (int)at_query.row_of(tid);
       len = row_length(p, b, &s);
       if (s < 0 || s >= p.g.slots) {
         atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);
@@ -786,7 +783,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   for (int i = lane; i < 16 * CH; i += 32) {
     const int r = wr + i / CH, c = i % CH, b = row_of[r];
     if (b < 0) continue;
-    const int h = kvh * p.per + (int)((m0 + r) % p.per);
+    const int h = kvh * p.per + at_query.head_of(r);
     *reinterpret_cast<uint4*>(static_cast<T*>(p.out) + b * p.o_row + h * p.o_head + c * 8) =
         *reinterpret_cast<const uint4*>(sm + tile_at<D>(r, c));
   }
@@ -794,7 +791,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   __syncwarp();
   for (int r = 0; r < 16; ++r)
     if (((r < 8 ? bad_a : bad_b) >> ((r & 7) * 4) & 0xf) && row_of[wr + r] >= 0)
-      row_again<T, D>(p, row_of[wr + r], kvh * p.per + (int)((m0 + wr + r) % p.per));
+      row_again<T, D>(p, row_of[wr + r], kvh * p.per + at_query.head_of(wr + r));
 }
 
 // Joins the ranges of each (row, head): a warp each, D / 32 dims per lane.

@@ -33,6 +33,16 @@ __device__ __forceinline__ int row_length(const SharedParams& p, int b, int* s) 
   return held_tokens(p.lengths[x], p.g.page_size, p.g.width);
 }
 
+// Queries of a key head in the order (row, head of the key head): the tile's first one
+// by 64-bit division once, those behind it by 32-bit ones.
+struct Queries {
+  long long row;   // row of the tile's first query
+  unsigned head, per;
+  __device__ __forceinline__ Queries(long long first, int per_) : row(first / per_), head((unsigned)(first % per_)), per(per_) {}
+  __device__ __forceinline__ long long row_of(int r) const { return row + (head + r) / per; }
+  __device__ __forceinline__ int head_of(int r) const { return (int)((head + r) % per); }
+};
+
 // Group of row b, by the whole warp: the last one that starts at or before b; -1
 // where b lies outside of them.
 __device__ __forceinline__ int row_group(const SharedParams& p, int b) {

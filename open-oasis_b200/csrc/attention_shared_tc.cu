@@ -59,6 +59,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   const int b0 = max(0, p.group_start[group]), b1 = min(p.rows, p.group_start[group + 1]);
   const long long queries = (long long)max(0, b1 - b0) * p.per, m0 = (long long)pair * 2 * kTile;
   if (m0 >= queries) return;  // the whole block
+  const Queries at_query(m0, p.per);
   const int P = p.g.page_size;
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -125,10 +126,10 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   // Q: the two tiles' rows, as TMA would lay them out
   for (int i = threadIdx.x; i < 2 * kTile * (D / 8); i += kSharedThreads) {
     const int r = i / (D / 8), ch = i % (D / 8);
-    const long long m = m0 + r;
     uint4 y = make_uint4(0, 0, 0, 0);
-    if (m < queries) {
-      const T* at = static_cast<const T*>(p.q) + (b0 + m / p.per) * p.q_row + (kvh * p.per + m % p.per) * p.q_head;
+    if (m0 + r < queries) {
+      const T* at = static_cast<const T*>(p.q) + (b0 + at_query.row_of(r)) * p.q_row +
+                    (kvh * p.per + at_query.head_of(r)) * p.q_head;
       y = *reinterpret_cast<const uint4*>(at + ch * 8);
     }
     *reinterpret_cast<uint4*>(sQ + (r / kTile) * C::TILE_BYTES + (ch / 8) * C::CHUNK_BYTES + tile_at<64>(r % kTile, ch % 8)) = y;
@@ -294,14 +295,15 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
     // ---------------- softmax and output ----------------
     const int t = warp >> 2, quarter = warp & 3;
-    const long long m_row = m0 + t * kTile + quarter * 32 + lane;  // this thread's query in the group
+    const int first_query = t * kTile + quarter * 32;  // of this warp, from the tiles' first one
+    const bool mine = m0 + first_query + lane < queries && t < tiles_here;
     const uint32_t lane_base = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_at = lane_base + C::S_COL + t * kTile, p_at = lane_base + C::P_COL + t * C::P_STEP,
                    o_at = lane_base + C::O_COL + t * D;
     int limit = 0;  // keys that the query sees
-    if (m_row < queries) {
+    if (mine) {
       int s;
-      limit = min(common, row_length(p, b0 + (int)(m_row / p.per), &s));
+      limit = min(common, row_length(p, b0 + (int)at_query.row_of(first_query + lane), &s));
     }
     const float sc = p.scale_log2;
     float m = -INFINITY, l = 0.f;
@@ -399,20 +401,22 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       if (lane == 0) mbar_arrive(&p_full[t]);
     }
     const int splits = p.prefix_splits + p.own_splits;
-    auto slot_of = [&](long long q) {  // range `split` of the group's query q
-      return ((b0 + q / p.per) * p.heads + kvh * p.per + q % p.per) * splits + split;
+    auto slot_of = [&](int r) {  // range `split` of the query r behind the warp's first one
+      return ((b0 + at_query.row_of(first_query + r)) * p.heads + kvh * p.per + at_query.head_of(first_query + r)) * splits + split;
     };
-    const bool mine = m_row < queries && t < tiles_here;
     if (blocks == 0) {
-      if (mine) p.part_ml[slot_of(m_row)] = make_float2(-INFINITY, 0.f);
+      if (mine) p.part_ml[slot_of(lane)] = make_float2(-INFINITY, 0.f);
     } else if (ok && wait_for(&pv_done[t], (blocks - 1) & 1, kDevTimeoutAccFull)) {
       tc_fence_after();
       if (m == -INFINITY && finite_f(l)) l = 0.f;  // no key that counts: masked ones left 2^-125 each
-      if (mine) p.part_ml[slot_of(m_row)] = make_float2(m, l);
+      if (mine) p.part_ml[slot_of(lane)] = make_float2(m, l);
       // O through this tile's Q, which no product reads any more: 32 columns of 32 rows,
       // so that a store covers four rows' 128 bytes
       const unsigned mine_rows = __ballot_sync(0xffffffffu, mine && !(m == -INFINITY && l == 0.f));
       uint8_t* stage = sQ + t * C::TILE_BYTES + quarter * (32 * 128);
+      long long to[8];  // this lane's rows of a store
+#pragma unroll
+      for (int i = 0; i < 8; ++i) to[i] = slot_of(i * 4 + (lane >> 3)) * D + (lane & 7) * 4;
 #pragma unroll
       for (int x = 0; x < D / 32; ++x) {
         uint32_t o[32];
@@ -426,8 +430,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
         for (int i = 0; i < 8; ++i) {
           const int r = i * 4 + (lane >> 3), ch = lane & 7;
           const uint4 y = *reinterpret_cast<const uint4*>(stage + tile_at<64>(r, ch));
-          if (mine_rows >> r & 1)
-            *reinterpret_cast<uint4*>(p.part_o + slot_of(m0 + t * kTile + quarter * 32 + r) * D + x * 32 + ch * 4) = y;
+          if (mine_rows >> r & 1) *reinterpret_cast<uint4*>(p.part_o + to[i] + x * 32) = y;
         }
         __syncwarp();
       }
