@@ -91,7 +91,8 @@ __device__ __forceinline__ void scores(const uint8_t* sk, int row0, const uint32
   }
 }
 
-template <typename T, int D>
+// RESCALE: O of the keys before first takes the factors fa and fb.
+template <typename T, int D, bool RESCALE = true>
 __device__ __forceinline__ void add_values(const uint8_t* sv, int row0, const uint32_t (&pa)[4], float fa, float fb,
                                            float (&o)[D / 8][4]) {
   const int lane = threadIdx.x & 31;
@@ -101,10 +102,12 @@ __device__ __forceinline__ void add_values(const uint8_t* sv, int row0, const ui
     ldsm_x4_t(b, sv + tile_at<D>(row0 + (lane & 15), t + (lane >> 4)));
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      o[t + u][0] *= fa;
-      o[t + u][1] *= fa;
-      o[t + u][2] *= fb;
-      o[t + u][3] *= fb;
+      if constexpr (RESCALE) {
+        o[t + u][0] *= fa;
+        o[t + u][1] *= fa;
+        o[t + u][2] *= fb;
+        o[t + u][3] *= fb;
+      }
       Elem<T>::mma(o[t + u], pa, b[2 * u], b[2 * u + 1]);
     }
   }
@@ -322,14 +325,15 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     pdl_wait();
     return;
   }
-  int s;
-  const int len = row_length(p, b, &s), P = p.g.page_size;
-  if (s < 0 || s >= p.g.slots) {
+  int s = p.seqs[b];  // on its way during the search
+  const int group = served_group(p, b), P = p.g.page_size;
+  const bool known = s >= 0 && s < p.g.slots;
+  const int len = known ? held_tokens(p.lengths[s], P, p.g.width) : 0;
+  const int begin = group_tokens(p, group);
+  if (!known) {
     if (lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);
     s = 0;
   }
-  const int group = served_group(p, b);
-  const int begin = group_tokens(p, group);
   const int units = len > begin ? (len - begin + kUnit - 1) / kUnit : 0;
   const int u0 = min(units, split * p.own_units), u1 = split + 1 < p.own_splits ? min(units, u0 + p.own_units) : units;
   if (split > 0 && u0 == units) {  // a shorter row has fewer ranges
@@ -519,11 +523,12 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
 
 // Prefix and own keys in one pass, for many rows with few keys each (forks of a short
 // prompt: a group per patch, a few frames behind it): 64 (row, head) queries of one key
-// head per block, whatever groups they belong to. Each group's prefix is read once for
-// the rows of the tile that are in it, then each warp goes through the own keys of its
-// 16 queries' rows, 16 keys at a time: the product is taken with all 16 queries and the
-// other rows' scores are masked, so that the softmax and O stay in one fragment and
-// nothing goes through memory in between.
+// head per block, whatever groups they belong to. First each warp goes through the own
+// keys of its 16 queries' rows, 16 keys at a time: the product is taken with all 16
+// queries and the other rows' scores are masked, so that the softmax and O stay in one
+// fragment; a row's first 16 keys find its O empty and need no rescaling. Then each
+// group's prefix is read once for the rows of the tile that are in it. Bound by issue:
+// about 200 instructions for each row's 16 keys, and by the latency of their loads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel(SharedParams p) {
   constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kPrefixKeys * D * 2, UNIT = kUnit * D * 2;
@@ -532,6 +537,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   __shared__ int seq_of[kPrefixRows];    // its sequence
   __shared__ int len_of[kPrefixRows];    // its tokens
   __shared__ int begin_of[kPrefixRows];  // its first own token
+  __shared__ int page_of[kPrefixRows];   // and that token's page
   __shared__ int group_of[kPrefixRows];
   __shared__ int near_starts[kThreads];  // group starts from the first query's group on
   __shared__ int lead_len[4], lead_row[4];
@@ -579,7 +585,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
     len_of[tid] = len;
     begin_of[tid] = begin;
     group_of[tid] = group;
+    page_of[tid] = len > begin ? p.table[(long long)s * p.g.width + begin / P] : -1;
   }
+  cp_async_wait_all();
   __syncthreads();
 
   const int wr = warp * 16, ra = wr + (lane >> 2), rb = ra + 8;
@@ -588,9 +596,11 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
 #pragma unroll
   for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
   Running run;
-  // one step of this warp's 16 queries with the 16 keys at rows `row` of a tile; query x
-  // of the tile sees keys below lim[x]
-  auto step = [&](const uint8_t* sk, const uint8_t* sv, int row, int key0, int lim_a, int lim_b) {
+#pragma unroll
+  for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
+  // one step of this warp's 16 queries with the 16 keys at rows `row` of a tile; the
+  // fragment's rows see keys below lim_a and lim_b; `fresh`: their O is still empty
+  auto step = [&](const uint8_t* sk, const uint8_t* sv, int row, int key0, int lim_a, int lim_b, bool fresh) {
     float x[2][4] = {};
     scores<T, D>(sk, row, qa, x);
 #pragma unroll
@@ -603,11 +613,76 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
     float fa, fb;
     uint32_t pa[4];
     softmax_step<T>(x, run, fa, fb, pa);
-    add_values<T, D>(sv, row, pa, fa, fb, o);
+    if (fresh)
+      add_values<T, D, false>(sv, row, pa, fa, fb, o);
+    else
+      add_values<T, D>(sv, row, pa, fa, fb, o);
   };
 
+  // ---- own keys: this warp's rows in turn, (first query x, unit u)
+  uint8_t* ring = sm + kPrefixRows * D * 2 + warp * 4 * UNIT;
+  auto units_of = [&](int x) {
+    const int own = len_of[x] - begin_of[x];
+    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
+  };
+  auto next_row = [&](int x) {  // the first query of the next row
+    const int b = row_of[x];
+    do ++x;
+    while (x < wr + 16 && row_of[x] == b);
+    return x;
+  };
+  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 16: none
+    while (x < wr + 16 && (row_of[x] < 0 || u >= units_of(x))) {
+      x = row_of[x] < 0 ? wr + 16 : next_row(x);
+      u = 0;
+    }
+  };
+  unsigned ok_bits = 0;
+  auto load = [&](int x, int u, int n) {
+    uint8_t* kd = ring + (n & 1) * 2 * UNIT;
+    const int t = begin_of[x] + u * kUnit, left = len_of[x] - t;
+    int page = page_of[x], slot = u * kUnit;  // a prefix is whole pages: own tokens begin with one
+    if (slot >= P) {
+      page = p.table[(long long)seq_of[x] * p.g.width + t / P];
+      slot %= P;
+    }
+    const bool ok = page_ok(page, p.g.pages);
+    ok_bits = (ok_bits & ~(1u << (n & 1))) | ((unsigned)ok << (n & 1));
+    if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+    const uint4* at = pool + (tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + slot * CH);
+#pragma unroll
+    for (int i = 0; i < kUnit * CH / 32; ++i) {
+      const int y = i * 32 + lane, r = y / CH, c = y % CH;
+      const bool in = ok && r < left;  // rows behind the sequence hold anything: zero instead
+      cp_async16(kd + tile_at<D>(r, c), at + y, in);
+      cp_async16(kd + UNIT + tile_at<D>(r, c), at + to_v + y, in);
+    }
+    cp_async_commit();
+  };
+  int x = wr, u = 0;
+  skip(x, u);
+  if (x < wr + 16) load(x, u, 0);
+  for (int n = 0; x < wr + 16; ++n) {
+    int nx = x, nu = u + 1;
+    skip(nx, nu);
+    if (nx < wr + 16) {
+      load(nx, nu, n + 1);
+      cp_async_wait<1>();
+    } else {
+      cp_async_wait<0>();
+    }
+    __syncwarp();
+    if (ok_bits >> (n & 1) & 1) {
+      const uint8_t* sk = ring + (n & 1) * 2 * UNIT;
+      const int b = row_of[x], len = len_of[x];
+      step(sk, sk + UNIT, 0, begin_of[x] + u * kUnit, row_of[ra] == b ? len : 0, row_of[rb] == b ? len : 0, u == 0);
+    }
+    __syncwarp();  // the stage may be loaded again
+    x = nx;
+    u = nu;
+  }
+  __syncthreads();  // the rings' place is the prefix tiles'
   // ---- prefixes: the groups of the tile's rows in turn
-  bool have_q = false;
   for (int x = 0; x < kPrefixRows;) {
     const int group = group_of[x];
     const int tokens = begin_of[x];
@@ -683,84 +758,14 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
         cp_async_wait<0>();
       }
       __syncthreads();
-      if (!have_q) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
-        have_q = true;
-      }
       const uint8_t* sk = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
       if (__any_sync(0xffffffffu, lim_a > 0 || lim_b > 0))
         for (int h = 0; h < min(4, units - j * 4); ++h)
-          if (unit_ok[j & 1][h]) step(sk, sk + TILE, h * kUnit, (j * 4 + h) * kUnit, lim_a, lim_b);
+          if (unit_ok[j & 1][h]) step(sk, sk + TILE, h * kUnit, (j * 4 + h) * kUnit, lim_a, lim_b, false);
       __syncthreads();
     }
     __syncthreads();  // lead_len is free again
     x = after;
-  }
-  cp_async_wait_all();
-  __syncthreads();  // Q is there, and the prefix tiles are free
-  if (!have_q) {
-#pragma unroll
-    for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
-  }
-
-  // ---- own keys: this warp's rows in turn, (first query x, unit u)
-  uint8_t* ring = sm + kPrefixRows * D * 2 + warp * 4 * UNIT;
-  auto units_of = [&](int x) {
-    const int own = len_of[x] - begin_of[x];
-    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
-  };
-  auto next_row = [&](int x) {  // the first query of the next row
-    const int b = row_of[x];
-    do ++x;
-    while (x < wr + 16 && row_of[x] == b);
-    return x;
-  };
-  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 16: none
-    while (x < wr + 16 && (row_of[x] < 0 || u >= units_of(x))) {
-      x = row_of[x] < 0 ? wr + 16 : next_row(x);
-      u = 0;
-    }
-  };
-  unsigned ok_bits = 0;
-  auto load = [&](int x, int u, int n) {
-    uint8_t* kd = ring + (n & 1) * 2 * UNIT;
-    const int t = begin_of[x] + u * kUnit, len = len_of[x];
-    const int page = p.table[(long long)seq_of[x] * p.g.width + t / P];
-    const bool ok = page_ok(page, p.g.pages);
-    ok_bits = (ok_bits & ~(1u << (n & 1))) | ((unsigned)ok << (n & 1));
-    if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
-    const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P) * CH;
-#pragma unroll
-    for (int i = 0; i < kUnit * CH / 32; ++i) {
-      const int y = i * 32 + lane, r = y / CH, c = y % CH;
-      const bool in = ok && t + r < len;  // rows behind the sequence hold anything: zero instead
-      cp_async16(kd + tile_at<D>(r, c), pool + at + y, in);
-      cp_async16(kd + UNIT + tile_at<D>(r, c), pool + at + to_v + y, in);
-    }
-    cp_async_commit();
-  };
-  int x = wr, u = 0;
-  skip(x, u);
-  if (x < wr + 16) load(x, u, 0);
-  for (int n = 0; x < wr + 16; ++n) {
-    int nx = x, nu = u + 1;
-    skip(nx, nu);
-    if (nx < wr + 16) {
-      load(nx, nu, n + 1);
-      cp_async_wait<1>();
-    } else {
-      cp_async_wait<0>();
-    }
-    __syncwarp();
-    if (ok_bits >> (n & 1) & 1) {
-      const uint8_t* sk = ring + (n & 1) * 2 * UNIT;
-      const int b = row_of[x], len = len_of[x];
-      step(sk, sk + UNIT, 0, begin_of[x] + u * kUnit, row_of[ra] == b ? len : 0, row_of[rb] == b ? len : 0);
-    }
-    __syncwarp();  // the stage may be loaded again
-    x = nx;
-    u = nu;
   }
   join_lanes(run);
 
