@@ -8,7 +8,7 @@
 // shared_prefix_kernel: the keys that a group's rows have in common, read once for all
 // of them: 64 (row, head) queries of one key head per block, 64 keys a step, mma.sync.
 // shared_own_kernel: each row's keys behind the prefix: four warps (or one) per (row, key
-// head, range), 16 keys a step, the heads of a key head as the 16 rows of a fragment.
+// head, range), 16 keys a step, the heads of a key head as the eight columns of a fragment.
 // Bound by reading the keys and values once. With one split it joins the prefix ranges too and
 // writes the result; otherwise shared_join_kernel does.
 #include "../../include/oasis_b200.h"
@@ -22,6 +22,7 @@ namespace {
 
 constexpr int kPrefixRows = 64;     // (row, head) queries of a block
 constexpr int kPrefixKeys = 64;     // keys of a step
+constexpr int kWholeRows = 32;      // queries of a block of the one-pass kernel
 constexpr int kThreads = 128;
 constexpr int kOwnWarps = 4;
 // Prefixes of at least this many tokens run on the tensor-memory kernel.
@@ -35,6 +36,10 @@ constexpr int kMostRanges = 2 * kMostSplits;
 template <int D>
 constexpr int prefix_smem() {
   return (kPrefixRows + 4 * kPrefixKeys) * D * 2;
+}
+template <int D>
+constexpr int whole_smem() {
+  return (kWholeRows + 4 * kPrefixKeys) * D * 2;  // Q, then two steps' K and V or four rings of two units
 }
 template <int D>
 constexpr int own_smem() {
@@ -91,8 +96,7 @@ __device__ __forceinline__ void scores(const uint8_t* sk, int row0, const uint32
   }
 }
 
-// RESCALE: O of the keys before first takes the factors fa and fb.
-template <typename T, int D, bool RESCALE = true>
+template <typename T, int D>
 __device__ __forceinline__ void add_values(const uint8_t* sv, int row0, const uint32_t (&pa)[4], float fa, float fb,
                                            float (&o)[D / 8][4]) {
   const int lane = threadIdx.x & 31;
@@ -102,12 +106,10 @@ __device__ __forceinline__ void add_values(const uint8_t* sv, int row0, const ui
     ldsm_x4_t(b, sv + tile_at<D>(row0 + (lane & 15), t + (lane >> 4)));
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      if constexpr (RESCALE) {
-        o[t + u][0] *= fa;
-        o[t + u][1] *= fa;
-        o[t + u][2] *= fb;
-        o[t + u][3] *= fb;
-      }
+      o[t + u][0] *= fa;
+      o[t + u][1] *= fa;
+      o[t + u][2] *= fb;
+      o[t + u][3] *= fb;
       Elem<T>::mma(o[t + u], pa, b[2 * u], b[2 * u + 1]);
     }
   }
@@ -277,6 +279,88 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
   }
 }
 
+// Steps of a warp with eight queries as the columns of the product and 16 keys as its
+// rows: a row of the batch has few heads to a key head, so that the other way round most
+// of a fragment's 16 query rows would be idle through the softmax. A lane holds columns
+// 2 (lane % 4) and the next of S^T (keys x queries) and of O^T (dims x queries).
+template <int D>
+struct Columns {
+  float m[2], l[2];  // l: this lane's keys' share until join()
+  float o[D / 16][4];
+  __device__ __forceinline__ Columns() {
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 16; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
+  }
+  __device__ __forceinline__ void join() {
+#pragma unroll
+    for (int w = 4; w < 32; w <<= 1) {
+      l[0] += __shfl_xor_sync(0xffffffffu, l[0], w);
+      l[1] += __shfl_xor_sync(0xffffffffu, l[1], w);
+    }
+  }
+};
+
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// The 16 keys at rows row0 of a tile, the first of them key `key0`; a column sees keys
+// below its limit. `fresh`: the columns that see any have no keys yet.
+template <typename T, int D>
+__device__ __forceinline__ void column_step(Columns<D>& c, const uint8_t* sk, const uint8_t* sv, int row0, int key0,
+                                            const uint32_t (&qb)[D / 16][2], int lim_a, int lim_b, bool fresh,
+                                            float scale_log2) {
+  const int lane = threadIdx.x & 31;
+  float x[4] = {};
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    uint32_t a[4];
+    ldsm_x4(a, sk + tile_at<D>(row0 + (lane & 15), s * 2 + (lane >> 4)));
+    Elem<T>::mma(x, a, qb[s][0], qb[s][1]);
+  }
+  const int key = key0 + (lane >> 2);
+  x[0] = key < lim_a ? x[0] * scale_log2 : -INFINITY;
+  x[1] = key < lim_b ? x[1] * scale_log2 : -INFINITY;
+  x[2] = key + 8 < lim_a ? x[2] * scale_log2 : -INFINITY;
+  x[3] = key + 8 < lim_b ? x[3] * scale_log2 : -INFINITY;
+  float na = fmaxf(x[0], x[2]), nb = fmaxf(x[1], x[3]);
+#pragma unroll
+  for (int w = 4; w < 32; w <<= 1) {
+    na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, w));
+    nb = fmaxf(nb, __shfl_xor_sync(0xffffffffu, nb, w));
+  }
+  na = fmaxf(na, c.m[0]);
+  nb = fmaxf(nb, c.m[1]);
+  const float sa = softmax_shift(na), sb = softmax_shift(nb);
+  const float fa = ex2_approx(c.m[0] - sa), fb = ex2_approx(c.m[1] - sb);
+  c.m[0] = na;
+  c.m[1] = nb;
+  x[0] = ex2_approx(x[0] - sa);
+  x[1] = ex2_approx(x[1] - sb);
+  x[2] = ex2_approx(x[2] - sa);
+  x[3] = ex2_approx(x[3] - sb);
+  c.l[0] = c.l[0] * fa + (x[0] + x[2]);
+  c.l[1] = c.l[1] * fb + (x[1] + x[3]);
+  // P^T (keys x queries) turned into the second operand: the one rounding inside the sum
+  const uint32_t b0 = transpose8(Elem<T>::pack(x[0], x[1])), b1 = transpose8(Elem<T>::pack(x[2], x[3]));
+#pragma unroll
+  for (int t = 0; t < D / 16; ++t) {
+    uint32_t a[4];
+    ldsm_x4_t(a, sv + tile_at<D>(row0 + (lane & 7) + ((lane >> 4) << 3), t * 2 + ((lane >> 3) & 1)));
+    if (!fresh) {
+      c.o[t][0] *= fa;
+      c.o[t][1] *= fb;
+      c.o[t][2] *= fa;
+      c.o[t][3] *= fb;
+    }
+    Elem<T>::mma(c.o[t], a, b0, b1);
+  }
+}
+
 // A row's result where the joined ranges are not finite: key by key, so that masked
 // places and the formula's own NaN come out as they should. Whole warp.
 template <typename T, int D>
@@ -304,7 +388,7 @@ __device__ __noinline__ void row_again(const SharedParams& p, int b, int h) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams p) {
-  constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kUnit * D * 2;
+  constexpr int CH = D / 8, KS = D / 16, MT = D / 16, TILE = kUnit * D * 2;
   extern __shared__ __align__(128) uint8_t sm[];
   // Behind a prefix kernel this one starts when every block of that one is past its own
   // wait, so that all before it is done; its ranges are waited for where they are joined.
@@ -342,7 +426,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   }
   const int* table = p.table + (long long)s * p.g.width;
   const uint4* pool = static_cast<const uint4*>(p.pool);
-  const int nh = min(16, p.per - ht * 16), h0 = kvh * p.per + ht * 16;  // heads of this fragment
+  const int nh = min(8, p.per - ht * 8), h0 = kvh * p.per + ht * 8;  // heads: the columns
 
   unsigned ok_bits = 0;  // of the two units in flight
   auto load = [&](int u, int n) {
@@ -365,20 +449,17 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   };
   if (u0 + member < u1) load(u0 + member, 0);
 
-  const int ra = lane >> 2;
+  const int ca = (lane & 3) * 2;  // this lane's columns: ca and ca + 1
   const T* q = static_cast<const T*>(p.q) + b * p.q_row + h0 * p.q_head;
-  uint32_t qa[KS][4];
+  uint32_t qb[KS][2];
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int r = ra + (e & 1) * 8, c = k * 16 + (e >> 1) * 8 + (lane & 3) * 2;
-      qa[k][e] = r < nh ? *reinterpret_cast<const uint32_t*>(q + r * p.q_head + c) : 0u;
+    for (int e = 0; e < 2; ++e) {
+      const int r = lane >> 2, c = k * 16 + e * 8 + (lane & 3) * 2;
+      qb[k][e] = r < nh ? *reinterpret_cast<const uint32_t*>(q + r * p.q_head + c) : 0u;
     }
-  float o[NT][4];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-  Running run;
+  Columns<D> run;
   for (int u = u0 + member, n = 0; u < u1; u += p.team, ++n) {
     if (u + p.team < u1) {
       load(u + p.team, n + 1);
@@ -389,89 +470,77 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     __syncwarp();
     if (ok_bits >> (n & 1) & 1) {
       const uint8_t* sk = ring + (n & 1) * 2 * TILE;
-      float sc[2][4] = {};
-      scores<T, D>(sk, 0, qa, sc);
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = begin + u * kUnit + t * 8 + (lane & 3) * 2 + (e & 1);
-          sc[t][e] = key < len ? sc[t][e] * p.scale_log2 : -INFINITY;
-        }
-      float fa, fb;
-      uint32_t pa[4];
-      softmax_step<T>(sc, run, fa, fb, pa);
-      add_values<T, D>(sk + TILE, 0, pa, fa, fb, o);
+      column_step<T, D>(run, sk, sk + TILE, 0, begin + u * kUnit, qb, len, len, n == 0, p.scale_log2);
     }
     __syncwarp();  // the stage may be loaded again
   }
-  join_lanes(run);
+  run.join();
 
   if (p.team > 1) {  // the team's sums, in fragment order, to its first warp
     float* mine = reinterpret_cast<float*>(ring) + lane;
     __shared__ float4 stats[kOwnWarps][32];
     if (member > 0) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < MT; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) mine[(t * 4 + e) * 32] = o[t][e];
-      stats[member][lane] = make_float4(run.ma, run.mb, run.la, run.lb);
+        for (int e = 0; e < 4; ++e) mine[(t * 4 + e) * 32] = run.o[t][e];
+      stats[member][lane] = make_float4(run.m[0], run.m[1], run.l[0], run.l[1]);
     }
     __syncthreads();
     if (member > 0) {
       pdl_wait();
       return;
     }
-    float ma = run.ma, mb = run.mb;
+    float ma = run.m[0], mb = run.m[1];
 #pragma unroll
     for (int w = 1; w < kOwnWarps; ++w) {
       ma = fmaxf(ma, stats[w][lane].x);
       mb = fmaxf(mb, stats[w][lane].y);
     }
     const float sa = softmax_shift(ma), sb = softmax_shift(mb);
-    const float ka = ex2_approx(run.ma - sa), kb = ex2_approx(run.mb - sb);
-    run.la *= ka;
-    run.lb *= kb;
+    const float ka = ex2_approx(run.m[0] - sa), kb = ex2_approx(run.m[1] - sb);
+    run.l[0] *= ka;
+    run.l[1] *= kb;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      o[t][0] *= ka;
-      o[t][1] *= ka;
-      o[t][2] *= kb;
-      o[t][3] *= kb;
+    for (int t = 0; t < MT; ++t) {
+      run.o[t][0] *= ka;
+      run.o[t][1] *= kb;
+      run.o[t][2] *= ka;
+      run.o[t][3] *= kb;
     }
 #pragma unroll
     for (int w = 1; w < kOwnWarps; ++w) {
       const float4 st = stats[w][lane];
       const float fa = ex2_approx(st.x - sa), fb = ex2_approx(st.y - sb);
-      run.la = fmaf(st.z, fa, run.la);
-      run.lb = fmaf(st.w, fb, run.lb);
+      run.l[0] = fmaf(st.z, fa, run.l[0]);
+      run.l[1] = fmaf(st.w, fb, run.l[1]);
       const float* other = reinterpret_cast<const float*>(sm + w * 4 * TILE) + lane;
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        o[t][0] = fmaf(other[(t * 4 + 0) * 32], fa, o[t][0]);
-        o[t][1] = fmaf(other[(t * 4 + 1) * 32], fa, o[t][1]);
-        o[t][2] = fmaf(other[(t * 4 + 2) * 32], fb, o[t][2]);
-        o[t][3] = fmaf(other[(t * 4 + 3) * 32], fb, o[t][3]);
+      for (int t = 0; t < MT; ++t) {
+        run.o[t][0] = fmaf(other[(t * 4 + 0) * 32], fa, run.o[t][0]);
+        run.o[t][1] = fmaf(other[(t * 4 + 1) * 32], fb, run.o[t][1]);
+        run.o[t][2] = fmaf(other[(t * 4 + 2) * 32], fa, run.o[t][2]);
+        run.o[t][3] = fmaf(other[(t * 4 + 3) * 32], fb, run.o[t][3]);
       }
     }
-    run.ma = ma;
-    run.mb = mb;
+    run.m[0] = ma;
+    run.m[1] = mb;
   }
 
   const int splits = p.prefix_splits + p.own_splits;
+  const int dim = lane >> 2;  // of a 16-dim tile: this one and the one eight behind it
   if (p.own_splits > 1) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int r = ra + half * 8;
-      if (r >= nh) continue;
-      const long long slot = ((long long)b * p.heads + h0 + r) * splits + p.prefix_splits + split;
-      const float mm = half ? run.mb : run.ma, ll = half ? run.lb : run.la;
-      if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm, ll);
-      if (mm == -INFINITY && ll == 0.f) continue;
+      if (ca + half >= nh) continue;
+      const long long slot = ((long long)b * p.heads + h0 + ca + half) * splits + p.prefix_splits + split;
+      if (dim == 0) p.part_ml[slot] = make_float2(run.m[half], run.l[half]);
+      if (run.m[half] == -INFINITY && run.l[half] == 0.f) continue;  // its sums are not read
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
-        *reinterpret_cast<float2*>(p.part_o + slot * D + t * 8 + (lane & 3) * 2) =
-            make_float2(o[t][2 * half], o[t][2 * half + 1]);
+      for (int t = 0; t < MT; ++t) {
+        p.part_o[slot * D + t * 16 + dim] = run.o[t][half];
+        p.part_o[slot * D + t * 16 + dim + 8] = run.o[t][half + 2];
+      }
     }
     pdl_wait();  // nobody ends before the prefix kernel does: what follows waits for this one alone
     return;
@@ -479,12 +548,12 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   // the prefix ranges of these heads join here
   pdl_wait();
   unsigned bad = 0;
+  float inv[2];
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const int r = ra + half * 8;
-    const bool mine = r < nh;
-    const long long slot = ((long long)b * p.heads + h0 + (mine ? r : 0)) * splits;
-    float m = half ? run.mb : run.ma, l = half ? run.lb : run.la;
+    const bool mine = ca + half < nh;
+    const long long slot = ((long long)b * p.heads + h0 + (mine ? ca + half : 0)) * splits;
+    float m = run.m[half], l = run.l[half];
     if (group >= 0 && mine) {
       for (int i = 0; i < p.prefix_splits; ++i) {
         const float2 ml = p.part_ml[slot + i];
@@ -493,52 +562,55 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
         const float fo = ex2_approx(m - sh), fp = ex2_approx(ml.x - sh);
         l = l * fo + ml.y * fp;
         m = n;
+        const float* y = p.part_o + (slot + i) * D + dim;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          const float2 y = *reinterpret_cast<const float2*>(p.part_o + (slot + i) * D + t * 8 + (lane & 3) * 2);
-          o[t][2 * half] = o[t][2 * half] * fo + y.x * fp;
-          o[t][2 * half + 1] = o[t][2 * half + 1] * fo + y.y * fp;
+        for (int t = 0; t < MT; ++t) {
+          run.o[t][half] = run.o[t][half] * fo + y[t * 16] * fp;
+          run.o[t][half + 2] = run.o[t][half + 2] * fo + y[t * 16 + 8] * fp;
         }
       }
     }
-    const float inv = len > 0 ? 1.f / l : 0.f;  // an empty sequence gives zeros
+    inv[half] = len > 0 ? 1.f / l : 0.f;  // an empty sequence gives zeros
     bool ok = len == 0 || (l > 0.f && finite_f(l));
-    T* out = static_cast<T*>(p.out) + b * p.o_row + (h0 + r) * p.o_head;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      ok = ok && finite_f(o[t][2 * half]) && finite_f(o[t][2 * half + 1]);
-      if (mine)
-        *reinterpret_cast<uint32_t*>(out + t * 8 + (lane & 3) * 2) =
-            Elem<T>::pack(o[t][2 * half] * inv, o[t][2 * half + 1] * inv);
-    }
+    for (int t = 0; t < MT; ++t) ok = ok && finite_f(run.o[t][half]) && finite_f(run.o[t][half + 2]);
     const unsigned votes = __ballot_sync(0xffffffffu, mine && !ok);
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (votes >> (4 * i) & 0xf) bad |= 1u << (half * 8 + i);
+    for (int i = 0; i < 4; ++i)
+      if (votes & (0x11111111u << i)) bad |= 1u << (2 * i + half);
   }
+  // O^T turned back, a pair of dims of query lane / 4 in a register
+  T* out = static_cast<T*>(p.out) + b * p.o_row + (h0 + (lane >> 2)) * p.o_head + ca;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const uint32_t y = transpose8(Elem<T>::pack(run.o[t][2 * e] * inv[0], run.o[t][2 * e + 1] * inv[1]));
+      if ((lane >> 2) < nh) *reinterpret_cast<uint32_t*>(out + t * 16 + e * 8) = y;
+    }
   __syncwarp();
   for (int r = 0; bad >> r; ++r)
     if (bad >> r & 1) row_again<T, D>(p, b, h0 + r);
 }
 
 // Prefix and own keys in one pass, for many rows with few keys each (forks of a short
-// prompt: a group per patch, a few frames behind it): 64 (row, head) queries of one key
+// prompt: a group per patch, a few frames behind it): 32 (row, head) queries of one key
 // head per block, whatever groups they belong to. First each warp goes through the own
-// keys of its 16 queries' rows, 16 keys at a time: the product is taken with all 16
-// queries and the other rows' scores are masked, so that the softmax and O stay in one
-// fragment; a row's first 16 keys find its O empty and need no rescaling. Then each
+// keys of its eight queries' rows, 16 keys at a time: the product is taken with all eight
+// and the other rows' scores are masked, so that the softmax and O stay in one fragment;
+// a row's first 16 keys find its O empty and need no rescaling. Then each
 // group's prefix is read once for the rows of the tile that are in it. Bound by issue:
 // about 200 instructions for each row's 16 keys, and by the latency of their loads.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel(SharedParams p) {
-  constexpr int CH = D / 8, KS = D / 16, NT = D / 8, TILE = kPrefixKeys * D * 2, UNIT = kUnit * D * 2;
+__global__ void __launch_bounds__(kThreads, D == 64 ? 6 : 3) shared_whole_kernel(SharedParams p) {
+  constexpr int CH = D / 8, KS = D / 16, MT = D / 16, TILE = kPrefixKeys * D * 2, UNIT = kUnit * D * 2;
   extern __shared__ __align__(128) uint8_t sm[];
-  __shared__ int row_of[kPrefixRows];    // row of a query, -1: none
-  __shared__ int seq_of[kPrefixRows];    // its sequence
-  __shared__ int len_of[kPrefixRows];    // its tokens
-  __shared__ int begin_of[kPrefixRows];  // its first own token
-  __shared__ int page_of[kPrefixRows];   // and that token's page
-  __shared__ int group_of[kPrefixRows];
+  __shared__ int row_of[kWholeRows];    // row of a query, -1: none
+  __shared__ int seq_of[kWholeRows];    // its sequence
+  __shared__ int len_of[kWholeRows];    // its tokens
+  __shared__ int begin_of[kWholeRows];  // its first own token
+  __shared__ int page_of[kWholeRows];   // and that token's page
+  __shared__ int group_of[kWholeRows];
   __shared__ int near_starts[kThreads];  // group starts from the first query's group on
   __shared__ int lead_len[4], lead_row[4];
   __shared__ int unit_ok[2][4];
@@ -546,13 +618,13 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   pdl_wait();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int kvh = blockIdx.x % p.g.kv_heads;
-  const long long m0 = (long long)(blockIdx.x / p.g.kv_heads) * kPrefixRows, queries = (long long)p.rows * p.per;
+  const long long m0 = (long long)(blockIdx.x / p.g.kv_heads) * kWholeRows, queries = (long long)p.rows * p.per;
   const Queries at_query(m0, p.per);
   const int P = p.g.page_size;
   const uint4* pool = static_cast<const uint4*>(p.pool);
   const long long to_v = p.g.kv_heads * tile_vectors(p.g);
   const T* q = static_cast<const T*>(p.q);
-  for (int i = tid; i < kPrefixRows * CH; i += kThreads) {
+  for (int i = tid; i < kWholeRows * CH; i += kThreads) {
     const int r = i / CH, c = i % CH;
     const bool ok = m0 + r < queries;
     const long long b = at_query.row_of(ok ? r : 0);
@@ -562,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   const int g0 = max(0, row_group(p, (int)at_query.row));
   near_starts[tid] = p.groups > 0 ? p.group_start[min(g0 + tid, p.groups)] : 0;
   __syncthreads();
-  if (tid < kPrefixRows) {
+  if (tid < kWholeRows) {
     int b = -1, s = 0, len = 0, group = -1, begin = 0;
     if (m0 + tid < queries) {
       b = (int)at_query.row_of(tid);
@@ -590,37 +662,21 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   cp_async_wait_all();
   __syncthreads();
 
-  const int wr = warp * 16, ra = wr + (lane >> 2), rb = ra + 8;
-  uint32_t qa[KS][4];
-  float o[NT][4];
+  const int wr = warp * 8, ca = wr + (lane & 3) * 2, cb = ca + 1;  // this warp's queries, this lane's columns
+  uint32_t qb[KS][2];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
-  Running run;
-#pragma unroll
-  for (int s = 0; s < KS; ++s) ldsm_x4(qa[s], sm + tile_at<D>(wr + (lane & 15), s * 2 + (lane >> 4)));
-  // one step of this warp's 16 queries with the 16 keys at rows `row` of a tile; the
-  // fragment's rows see keys below lim_a and lim_b; `fresh`: their O is still empty
-  auto step = [&](const uint8_t* sk, const uint8_t* sv, int row, int key0, int lim_a, int lim_b, bool fresh) {
-    float x[2][4] = {};
-    scores<T, D>(sk, row, qa, x);
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int key = key0 + t * 8 + (lane & 3) * 2 + (e & 1);
-        x[t][e] = key < (e < 2 ? lim_a : lim_b) ? x[t][e] * p.scale_log2 : -INFINITY;
-      }
-    float fa, fb;
-    uint32_t pa[4];
-    softmax_step<T>(x, run, fa, fb, pa);
-    if (fresh)
-      add_values<T, D, false>(sv, row, pa, fa, fb, o);
-    else
-      add_values<T, D>(sv, row, pa, fa, fb, o);
-  };
+  for (int s = 0; s < KS; s += 2) {
+    uint32_t r[4];
+    ldsm_x4(r, sm + tile_at<D>(wr + (lane & 7), s * 2 + (lane >> 3)));
+    qb[s][0] = r[0];
+    qb[s][1] = r[1];
+    qb[s + 1][0] = r[2];
+    qb[s + 1][1] = r[3];
+  }
+  Columns<D> run;
 
   // ---- own keys: this warp's rows in turn, (first query x, unit u)
-  uint8_t* ring = sm + kPrefixRows * D * 2 + warp * 4 * UNIT;
+  uint8_t* ring = sm + kWholeRows * D * 2 + warp * 4 * UNIT;
   auto units_of = [&](int x) {
     const int own = len_of[x] - begin_of[x];
     return own > 0 ? (own + kUnit - 1) / kUnit : 0;
@@ -628,12 +684,12 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   auto next_row = [&](int x) {  // the first query of the next row
     const int b = row_of[x];
     do ++x;
-    while (x < wr + 16 && row_of[x] == b);
+    while (x < wr + 8 && row_of[x] == b);
     return x;
   };
-  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 16: none
-    while (x < wr + 16 && (row_of[x] < 0 || u >= units_of(x))) {
-      x = row_of[x] < 0 ? wr + 16 : next_row(x);
+  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 8: none
+    while (x < wr + 8 && (row_of[x] < 0 || u >= units_of(x))) {
+      x = row_of[x] < 0 ? wr + 8 : next_row(x);
       u = 0;
     }
   };
@@ -661,11 +717,11 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   };
   int x = wr, u = 0;
   skip(x, u);
-  if (x < wr + 16) load(x, u, 0);
-  for (int n = 0; x < wr + 16; ++n) {
+  if (x < wr + 8) load(x, u, 0);
+  for (int n = 0; x < wr + 8; ++n) {
     int nx = x, nu = u + 1;
     skip(nx, nu);
-    if (nx < wr + 16) {
+    if (nx < wr + 8) {
       load(nx, nu, n + 1);
       cp_async_wait<1>();
     } else {
@@ -675,7 +731,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
     if (ok_bits >> (n & 1) & 1) {
       const uint8_t* sk = ring + (n & 1) * 2 * UNIT;
       const int b = row_of[x], len = len_of[x];
-      step(sk, sk + UNIT, 0, begin_of[x] + u * kUnit, row_of[ra] == b ? len : 0, row_of[rb] == b ? len : 0, u == 0);
+      column_step<T, D>(run, sk, sk + UNIT, 0, begin_of[x] + u * kUnit, qb, row_of[ca] == b ? len : 0,
+                        row_of[cb] == b ? len : 0, u == 0, p.scale_log2);
     }
     __syncwarp();  // the stage may be loaded again
     x = nx;
@@ -683,14 +740,14 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   }
   __syncthreads();  // the rings' place is the prefix tiles'
   // ---- prefixes: the groups of the tile's rows in turn
-  for (int x = 0; x < kPrefixRows;) {
+  for (int x = 0; x < kWholeRows;) {
     const int group = group_of[x];
     const int tokens = begin_of[x];
     if (row_of[x] < 0) break;
     // the rows of the group are consecutive
     int after = x;
 #pragma unroll
-    for (int i = 0; i < kPrefixRows; i += 32)
+    for (int i = 0; i < kWholeRows; i += 32)
       after += __popc(__ballot_sync(0xffffffffu, i + lane >= x && group_of[i + lane] == group && row_of[i + lane] >= 0));
     if (tokens == 0) {
       x = after;
@@ -730,7 +787,7 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
     const int* lead = p.table + (long long)(len > 0 ? p.seqs[row] : 0) * p.g.width;
     const int units = (common + kUnit - 1) / kUnit, steps = (units + 3) / 4;
     auto load = [&](int j) {
-      uint8_t* kd = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+      uint8_t* kd = sm + kWholeRows * D * 2 + (j & 1) * 2 * TILE;
       const int keys = min(4, units - j * 4) * kUnit;
       for (int i = tid; i < keys * CH; i += kThreads) {
         const int r = i / CH, c = i % CH;
@@ -748,8 +805,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
       cp_async_commit();
     };
     if (steps > 0) load(0);
-    const int lim_a = ra >= x && ra < after ? min(common, len_of[ra]) : 0;
-    const int lim_b = rb >= x && rb < after ? min(common, len_of[rb]) : 0;
+    const int lim_a = ca >= x && ca < after ? min(common, len_of[ca]) : 0;
+    const int lim_b = cb >= x && cb < after ? min(common, len_of[cb]) : 0;
     for (int j = 0; j < steps; ++j) {
       if (j + 1 < steps) {
         load(j + 1);
@@ -758,34 +815,36 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
         cp_async_wait<0>();
       }
       __syncthreads();
-      const uint8_t* sk = sm + kPrefixRows * D * 2 + (j & 1) * 2 * TILE;
+      const uint8_t* sk = sm + kWholeRows * D * 2 + (j & 1) * 2 * TILE;
       if (__any_sync(0xffffffffu, lim_a > 0 || lim_b > 0))
         for (int h = 0; h < min(4, units - j * 4); ++h)
-          if (unit_ok[j & 1][h]) step(sk, sk + TILE, h * kUnit, (j * 4 + h) * kUnit, lim_a, lim_b, false);
+          if (unit_ok[j & 1][h])
+            column_step<T, D>(run, sk, sk + TILE, h * kUnit, (j * 4 + h) * kUnit, qb, lim_a, lim_b, false, p.scale_log2);
       __syncthreads();
     }
     __syncthreads();  // lead_len is free again
     x = after;
   }
-  join_lanes(run);
+  run.join();
 
-  // ---- result, through this warp's own rows of Q
-  const float ia = len_of[ra] > 0 ? 1.f / run.la : 0.f, ib = len_of[rb] > 0 ? 1.f / run.lb : 0.f;
-  bool ok_a = len_of[ra] == 0 || (run.la > 0.f && finite_f(run.la));
-  bool ok_b = len_of[rb] == 0 || (run.lb > 0.f && finite_f(run.lb));
+  // ---- result, O^T turned back through this warp's own rows of Q
+  const float ia = len_of[ca] > 0 ? 1.f / run.l[0] : 0.f, ib = len_of[cb] > 0 ? 1.f / run.l[1] : 0.f;
+  bool ok_a = len_of[ca] == 0 || (run.l[0] > 0.f && finite_f(run.l[0]));
+  bool ok_b = len_of[cb] == 0 || (run.l[1] > 0.f && finite_f(run.l[1]));
+  const int qr = wr + (lane >> 2);
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    ok_a = ok_a && finite_f(o[t][0]) && finite_f(o[t][1]);
-    ok_b = ok_b && finite_f(o[t][2]) && finite_f(o[t][3]);
-    const int c = t ^ (ra & 7);  // ra and rb have the same low bits
-    uint8_t* at = sm + ra * (D * 2) + (c << 4) + (lane & 3) * 4;
-    *reinterpret_cast<uint32_t*>(at) = Elem<T>::pack(o[t][0] * ia, o[t][1] * ia);
-    *reinterpret_cast<uint32_t*>(at + 8 * D * 2) = Elem<T>::pack(o[t][2] * ib, o[t][3] * ib);
+  for (int t = 0; t < MT; ++t) {
+    ok_a = ok_a && finite_f(run.o[t][0]) && finite_f(run.o[t][2]);
+    ok_b = ok_b && finite_f(run.o[t][1]) && finite_f(run.o[t][3]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      *reinterpret_cast<uint32_t*>(sm + tile_at<D>(qr, t * 2 + e) + (lane & 3) * 4) =
+          transpose8(Elem<T>::pack(run.o[t][2 * e] * ia, run.o[t][2 * e + 1] * ib));
   }
   const unsigned bad_a = __ballot_sync(0xffffffffu, !ok_a), bad_b = __ballot_sync(0xffffffffu, !ok_b);
   __syncwarp();
 #pragma unroll
-  for (int i = lane; i < 16 * CH; i += 32) {
+  for (int i = lane; i < 8 * CH; i += 32) {
     const int r = wr + i / CH, c = i % CH, b = row_of[r];
     if (b < 0) continue;
     const int h = kvh * p.per + at_query.head_of(r);
@@ -794,8 +853,8 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 5 : 2) shared_whole_kernel
   }
   if ((bad_a | bad_b) == 0) return;
   __syncwarp();
-  for (int r = 0; r < 16; ++r)
-    if (((r < 8 ? bad_a : bad_b) >> ((r & 7) * 4) & 0xf) && row_of[wr + r] >= 0)
+  for (int r = 0; r < 8; ++r)
+    if (((r & 1 ? bad_b : bad_a) & (0x11111111u << (r >> 1))) && row_of[wr + r] >= 0)
       row_again<T, D>(p, row_of[wr + r], kvh * p.per + at_query.head_of(wr + r));
 }
 
@@ -885,7 +944,7 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const int sms = num_sms();
   const int K = a->cache->kv_heads;
   p->per = a->heads / K;
-  p->head_tiles = (p->per + 15) / 16;
+  p->head_tiles = (p->per + 7) / 8;
   const bool prefix = a->groups > 0 && a->prefix_pages_hint > 0;
   const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
   p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);
@@ -927,11 +986,11 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   p->team = units > 2 ? kOwnWarps : 1;
   p->own_units = (int)each;
   p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
-  // One pass where its blocks fill the GPU and a warp has at most 64 steps of own keys
-  // for its 16 queries and 16 of a prefix, one behind the other.
-  const long long blocks = ((long long)a->rows * p->per + kPrefixRows - 1) / kPrefixRows * K;
-  const long long rows = (16 + p->per - 1) / p->per, steps = rows * ((own + kUnit - 1) / kUnit);
-  p->whole = blocks >= 2LL * sms && steps <= 64 &&
+  // One pass where its blocks fill the GPU and a warp has at most 32 steps of own keys
+  // for its eight queries and 16 of a prefix, one behind the other.
+  const long long blocks = ((long long)a->rows * p->per + kWholeRows - 1) / kWholeRows * K;
+  const long long rows = (8 + p->per - 1) / p->per, steps = rows * ((own + kUnit - 1) / kUnit);
+  p->whole = blocks >= 4LL * sms && steps <= 32 &&
              (!prefix || (long long)a->prefix_pages_hint * a->cache->page_size <= 16 * kPrefixKeys);
 }
 
@@ -950,15 +1009,15 @@ int launch(const SharedParams& p, cudaStream_t s) {
     cudaError_t e =
         cudaFuncSetAttribute(shared_prefix_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<D>());
     if (e == cudaSuccess)
-      e = cudaFuncSetAttribute(shared_whole_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, prefix_smem<D>());
+      e = cudaFuncSetAttribute(shared_whole_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, whole_smem<D>());
     if (e == cudaSuccess)
       e = cudaFuncSetAttribute(shared_own_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, own_smem<D>());
     if (e != cudaSuccess) return set_error(OASIS_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
     attr[dev & 63] = true;
   }
   if (p.whole) {
-    const long long blocks = ((long long)p.rows * p.per + kPrefixRows - 1) / kPrefixRows * p.g.kv_heads;
-    launch_pdl(shared_whole_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), prefix_smem<D>(), s, p);
+    const long long blocks = ((long long)p.rows * p.per + kWholeRows - 1) / kWholeRows * p.g.kv_heads;
+    launch_pdl(shared_whole_kernel<T, D>, dim3((unsigned)blocks), dim3(kThreads), whole_smem<D>(), s, p);
     return check_launch("shared_whole_kernel");
   }
   if (p.prefix_splits && p.tensor) {
