@@ -675,68 +675,75 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 6 : 3) shared_whole_kernel
   }
   Columns<D> run;
 
-  // ---- own keys: this warp's rows in turn, (first query x, unit u)
+  // ---- own keys: this warp's rows in turn. Lane x % 8 holds what query x's row needs.
   uint8_t* ring = sm + kWholeRows * D * 2 + warp * 4 * UNIT;
-  auto units_of = [&](int x) {
-    const int own = len_of[x] - begin_of[x];
-    return own > 0 ? (own + kUnit - 1) / kUnit : 0;
+  const int qx = wr + (lane & 7), row_x = row_of[qx], len_x = len_of[qx], begin_x = begin_of[qx], page_x = page_of[qx];
+  const bool leads = row_x >= 0 && (qx == wr || row_of[qx - 1] != row_x);  // the row's first query in this warp
+  const int units_x = leads && len_x > begin_x ? (len_x - begin_x + kUnit - 1) / kUnit : 0;
+  const long long at_x = page_ok(page_x, p.g.pages) ? tile_offset(p.g, page_x, p.layer, 0, kvh) : -1;
+  const int row_a = row_of[ca], row_b = row_of[cb];
+  unsigned todo = __ballot_sync(0xffffffffu, lane < 8 && units_x > 0);
+  struct Step {
+    int row, len, key;  // the row, its tokens, the first of the 16 keys
+    bool fresh, there;
   };
-  auto next_row = [&](int x) {  // the first query of the next row
-    const int b = row_of[x];
-    do ++x;
-    while (x < wr + 8 && row_of[x] == b);
-    return x;
-  };
-  auto skip = [&](int& x, int& u) {  // to the first (x, u) at or behind it that holds keys; x = wr + 8: none
-    while (x < wr + 8 && (row_of[x] < 0 || u >= units_of(x))) {
-      x = row_of[x] < 0 ? wr + 8 : next_row(x);
-      u = 0;
-    }
-  };
-  unsigned ok_bits = 0;
-  auto load = [&](int x, int u, int n) {
+  int x = 0, u = 0, units = 0;  // where the loads are
+  long long at_first = 0;
+  Step next = {-1, 0, 0, true, false};
+  auto load = [&](int n) {
     uint8_t* kd = ring + (n & 1) * 2 * UNIT;
-    const int t = begin_of[x] + u * kUnit, left = len_of[x] - t;
-    int page = page_of[x], slot = u * kUnit;  // a prefix is whole pages: own tokens begin with one
+    next.key += u ? kUnit : 0;
+    next.fresh = u == 0;
+    int slot = u * kUnit;  // a prefix is whole pages: own tokens begin with one
+    long long at = at_first;
     if (slot >= P) {
-      page = p.table[(long long)seq_of[x] * p.g.width + t / P];
+      const int page = p.table[(long long)seq_of[wr + x] * p.g.width + next.key / P];
       slot %= P;
+      at = page_ok(page, p.g.pages) ? tile_offset(p.g, page, p.layer, 0, kvh) : -1;
     }
-    const bool ok = page_ok(page, p.g.pages);
-    ok_bits = (ok_bits & ~(1u << (n & 1))) | ((unsigned)ok << (n & 1));
-    if (!ok && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
-    const uint4* at = pool + (tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + slot * CH);
+    next.there = at >= 0;
+    if (!next.there && lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
+    const uint4* from = pool + (next.there ? at + slot * CH : 0) + lane;
+    const int left = next.there ? next.len - next.key : 0;  // rows behind the sequence hold anything: zero instead
 #pragma unroll
     for (int i = 0; i < kUnit * CH / 32; ++i) {
       const int y = i * 32 + lane, r = y / CH, c = y % CH;
-      const bool in = ok && r < left;  // rows behind the sequence hold anything: zero instead
-      cp_async16(kd + tile_at<D>(r, c), at + y, in);
-      cp_async16(kd + UNIT + tile_at<D>(r, c), at + to_v + y, in);
+      cp_async16(kd + tile_at<D>(r, c), from + i * 32, r < left);
+      cp_async16(kd + UNIT + tile_at<D>(r, c), from + to_v + i * 32, r < left);
     }
     cp_async_commit();
   };
-  int x = wr, u = 0;
-  skip(x, u);
-  if (x < wr + 8) load(x, u, 0);
-  for (int n = 0; x < wr + 8; ++n) {
-    int nx = x, nu = u + 1;
-    skip(nx, nu);
-    if (nx < wr + 8) {
-      load(nx, nu, n + 1);
+  auto advance = [&]() {  // to the next 16 keys; false behind the last ones
+    if (++u < units) return true;
+    if (!todo) return false;
+    x = __ffs(todo) - 1;
+    todo &= todo - 1;
+    u = 0;
+    units = __shfl_sync(0xffffffffu, units_x, x);
+    at_first = __shfl_sync(0xffffffffu, at_x, x);
+    next.row = __shfl_sync(0xffffffffu, row_x, x);
+    next.len = __shfl_sync(0xffffffffu, len_x, x);
+    next.key = __shfl_sync(0xffffffffu, begin_x, x);
+    return true;
+  };
+  bool more = advance();
+  if (more) load(0);
+  for (int n = 0; more; ++n) {
+    const Step now = next;
+    more = advance();
+    if (more) {
+      load(n + 1);
       cp_async_wait<1>();
     } else {
       cp_async_wait<0>();
     }
     __syncwarp();
-    if (ok_bits >> (n & 1) & 1) {
+    if (now.there) {
       const uint8_t* sk = ring + (n & 1) * 2 * UNIT;
-      const int b = row_of[x], len = len_of[x];
-      column_step<T, D>(run, sk, sk + UNIT, 0, begin_of[x] + u * kUnit, qb, row_of[ca] == b ? len : 0,
-                        row_of[cb] == b ? len : 0, u == 0, p.scale_log2);
+      column_step<T, D>(run, sk, sk + UNIT, 0, now.key, qb, row_a == now.row ? now.len : 0, row_b == now.row ? now.len : 0,
+                        now.fresh, p.scale_log2);
     }
     __syncwarp();  // the stage may be loaded again
-    x = nx;
-    u = nu;
   }
   __syncthreads();  // the rings' place is the prefix tiles'
   // ---- prefixes: the groups of the tile's rows in turn
