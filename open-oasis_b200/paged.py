@@ -30,41 +30,87 @@ STATUS = {
 }
 
 
-def _check_ints(t: torch.Tensor, name: str, device, numel: int | None = None):
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dtype != torch.int32 or not t.is_contiguous():
+# The calls take a few microseconds: what is right is found with few questions, and only
+# what is wrong is looked at closely.
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _on(stream, index: int) -> int:
+    """The stream handle of a call: `stream`, or the device's current one."""
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(index)
+    return _stream(stream)
+
+
+def _ints(t: torch.Tensor, name: str, index: int, numel: int) -> int:
+    """Address of a contiguous int32 tensor of `numel` values on device `index`."""
+    if t.dtype is torch.int32 and t.get_device() == index and t.numel() == numel and t.is_contiguous():
+        return t.data_ptr()
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on CUDA device {index}, got {t.device}")
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous int32")
-    if numel is not None and t.numel() != numel:
-        raise ValueError(f"{name} must hold {numel} values, got {t.numel()}")
+    raise ValueError(f"{name} must hold {numel} values, got {t.numel()}")
 
 
-def _check_device(device):
+def _check_device(index: int):
     """The library launches on the current device."""
-    if device.type != "cuda":
+    if index < 0:
         raise ValueError("tensors must be on a CUDA device")
-    if device.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {device}, but cuda:{torch.cuda.current_device()} is the current device")
+    if index != torch.cuda.current_device():
+        raise ValueError(f"tensors are on cuda:{index}, but cuda:{torch.cuda.current_device()} is the current device")
 
 
-def _check_rows(t: torch.Tensor, name: str, dtype, device, heads: int | None, dim: int):
-    """[rows, heads, dim] with contiguous, 16-byte aligned head vectors."""
-    if t.device != device:
-        raise ValueError(f"{name} must be on {device}, got {t.device}")
-    if t.dtype != dtype:
+def _rows(t: torch.Tensor, name: str, dtype, index: int, rows: int | None, heads: int | None, dim: int):
+    """(rows, heads, address, row stride, head stride) of a [rows, heads, dim] tensor with
+    contiguous, 16-byte aligned head vectors. Strides of dimensions of size one, which
+    torch leaves open, are those of packed rows."""
+    if t.dtype is dtype and t.get_device() == index and t.dim() == 3:
+        n, h, d = t.shape
+        if d == dim and (heads is None or h == heads) and (rows is None or n == rows):
+            row, head, one = t.stride()
+            if h == 1:
+                head = dim
+            if n <= 1:
+                row = h * dim
+            at = t.data_ptr()
+            if one == 1 and not (at & 15 or (row | head) & 7):
+                return n, h, at, row, head
+    if t.get_device() != index:
+        raise ValueError(f"{name} must be on CUDA device {index}, got {t.device}")
+    if t.dtype is not dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    want = f"[{'rows' if rows is None else rows}, {'heads' if heads is None else heads}, {dim}]"
     if t.dim() != 3 or t.shape[2] != dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [rows, {'heads' if heads is None else heads}, {dim}], got {tuple(t.shape)}")
+        raise ValueError(f"{name} must be {want}, got {tuple(t.shape)}")
+    if rows is not None and t.shape[0] != rows:
+        raise ValueError(f"{name} has {t.shape[0]} rows, not {rows}")
     if t.stride(2) != 1:
         raise ValueError(f"{name}: the values of a head must be contiguous")
-    if t.data_ptr() % 16 or any(t.stride(d) % 8 for d in (0, 1) if t.shape[d] > 1):
-        raise ValueError(f"{name}: head vectors must be 16-byte aligned (strides multiples of 8 elements)")
+    raise ValueError(f"{name}: head vectors must be 16-byte aligned (strides multiples of 8 elements)")
 
 
-def _strides(t: torch.Tensor) -> tuple[int, int]:
-    """Row and head strides; those of dimensions of size one are replaced by packed ones."""
-    head = t.stride(1) if t.shape[1] > 1 else t.shape[2]
-    return (t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]), head
+def _new(t: torch.Tensor, shape, stream) -> torch.Tensor:
+    """An output of a call on `stream`."""
+    out = t.new_empty(shape)
+    if stream is not None:
+        out.record_stream(stream)
+    return out
+
+
+_MOST = (1 << 31) - 1
+_void, _int, _long, _packed = C.c_void_p, C.c_int, C.c_longlong, C.c_char_p
+_reserve = _lib.packed_call("oasis_pages_reserve", _packed, _void, _void, _int, _void, _void)
+_write = _lib.packed_call("oasis_pages_write", _packed, _int, _void, _void, _long, _long, _long, _long, _void, _void,
+                          _void, _int, _int, _void)
+_fork = _lib.packed_call("oasis_pages_fork", _packed, _void, _void, _int, _int, _void)
+_free = _lib.packed_call("oasis_pages_free", _packed, _void, _int, _void)
+_compact = _lib.packed_call("oasis_pages_compact", _packed, _void)
+_prompt = _lib.packed_call("oasis_attention_prompt", _packed, _void)
+_shared = _lib.packed_call("oasis_attention_shared", _packed, _void)
+_pack_prompt = _lib.packer(_lib.OasisPromptArgs).pack
+_pack_shared = _lib.packer(_lib.OasisSharedArgs).pack
 
 
 class PagedCache:
@@ -97,70 +143,60 @@ class PagedCache:
             raise ValueError("pool must be a CUDA tensor")
         if table.dim() != 2:
             raise ValueError("table must be [sequences, max_pages]")
-        self.device = pool.device
-        _check_ints(table, "table", self.device)
-        _check_ints(lengths, "lengths", self.device, table.shape[0])
-        _check_ints(refs, "refs", self.device, pool.shape[0])
+        self.device, index = pool.device, pool.get_device()
+        _ints(table, "table", index, table.numel())
+        _ints(lengths, "lengths", index, table.shape[0])
+        _ints(refs, "refs", index, pool.shape[0])
         self.pool, self.table, self.lengths, self.refs = pool, table, lengths, refs
         self.pages, self.layers, _, self.kv_heads, self.page_size, self.head_dim = pool.shape
         self.sequences, self.max_pages = table.shape
-        self.dtype = pool.dtype
+        self.dtype, self._index = pool.dtype, index
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.ws = workspace(_lib.load().oasis_pages_workspace_size(self.pages, self.sequences), self.device)
-        self._c = _lib.OasisPageCache(pool.data_ptr(), self.pages, self.layers, self.kv_heads, self.page_size,
-                                      self.head_dim, DTYPES[self.dtype], table.data_ptr(), self.sequences,
-                                      self.max_pages, lengths.data_ptr(), refs.data_ptr(), self.status.data_ptr(),
-                                      self.ws.data_ptr(), self.ws.numel())
-        self._ref = C.byref(self._c)
+        c = _lib.OasisPageCache(pool.data_ptr(), self.pages, self.layers, self.kv_heads, self.page_size, self.head_dim,
+                                DTYPES[self.dtype], table.data_ptr(), self.sequences, self.max_pages, lengths.data_ptr(),
+                                refs.data_ptr(), self.status.data_ptr(), self.ws.data_ptr(), self.ws.numel())
+        self._c = bytes(c)  # the C struct, kept alive and passed as it is
+        self._at = C.cast(self._c, C.c_void_p).value
 
     def reserve(self, seqs: torch.Tensor, cu: torch.Tensor, stream=None) -> torch.Tensor:
         """Room for cu[i + 1] - cu[i] more tokens behind sequence seqs[i]; returns
         each one's length before (-1: refused, see `status`), for `write`."""
-        _check_device(self.device)
-        _check_ints(seqs, "seqs", self.device)
-        _check_ints(cu, "cu", self.device, seqs.numel() + 1)
-        start = torch.empty(seqs.shape, dtype=torch.int32, device=self.device)
-        if stream is not None:
-            start.record_stream(stream)
-        _lib.call("oasis_pages_reserve", self._ref, seqs.data_ptr(), cu.data_ptr(), seqs.numel(), start.data_ptr(),
-                  _stream(stream))
+        index, n = self._index, seqs.numel()
+        _check_device(index)
+        start = _new(seqs, n, stream)
+        _reserve(self._c, _ints(seqs, "seqs", index, n), _ints(cu, "cu", index, n + 1), n, start.data_ptr(),
+                 _on(stream, index))
         return start
 
     def write(self, layer: int, k: torch.Tensor, v: torch.Tensor, seqs: torch.Tensor, cu: torch.Tensor,
               start: torch.Tensor, stream=None):
         """Keys and values [rows, kv_heads, head_dim] of the reserved tokens: packed rows
         [cu[i], cu[i + 1]) belong to sequence seqs[i], from position start[i] on."""
-        _check_device(self.device)
-        _check_rows(k, "k", self.dtype, self.device, self.kv_heads, self.head_dim)
-        _check_rows(v, "v", self.dtype, self.device, self.kv_heads, self.head_dim)
-        if k.shape[0] != v.shape[0]:
-            raise ValueError(f"k has {k.shape[0]} rows and v {v.shape[0]}")
-        n = seqs.numel()
-        _check_ints(seqs, "seqs", self.device)
-        _check_ints(cu, "cu", self.device, n + 1)
-        _check_ints(start, "start", self.device, n)
-        _lib.call("oasis_pages_write", self._ref, layer, k.data_ptr(), v.data_ptr(), *_strides(k), *_strides(v),
-                  seqs.data_ptr(), cu.data_ptr(), start.data_ptr(), n, k.shape[0], _stream(stream))
+        index, n = self._index, seqs.numel()
+        _check_device(index)
+        rows, _, k_at, k_row, k_head = _rows(k, "k", self.dtype, index, None, self.kv_heads, self.head_dim)
+        _, _, v_at, v_row, v_head = _rows(v, "v", self.dtype, index, rows, self.kv_heads, self.head_dim)
+        _write(self._c, layer, k_at, v_at, k_row, k_head, v_row, v_head, _ints(seqs, "seqs", index, n),
+               _ints(cu, "cu", index, n + 1), _ints(start, "start", index, n), n, rows, _on(stream, index))
 
     def fork(self, src: torch.Tensor, dst: torch.Tensor, deep: bool = False, stream=None):
         """The empty sequences dst[i] continue src[i]: whole pages are shared and a
         partial last page is copied; deep=True copies every page."""
-        _check_device(self.device)
-        _check_ints(src, "src", self.device)
-        _check_ints(dst, "dst", self.device, src.numel())
-        _lib.call("oasis_pages_fork", self._ref, src.data_ptr(), dst.data_ptr(), src.numel(), int(deep),
-                  _stream(stream))
+        index, n = self._index, src.numel()
+        _check_device(index)
+        _fork(self._c, _ints(src, "src", index, n), _ints(dst, "dst", index, n), n, int(deep), _on(stream, index))
 
     def free(self, seqs: torch.Tensor, stream=None):
         """Empties sequences; their pages are free once nobody else holds them."""
-        _check_device(self.device)
-        _check_ints(seqs, "seqs", self.device)
-        _lib.call("oasis_pages_free", self._ref, seqs.data_ptr(), seqs.numel(), _stream(stream))
+        index, n = self._index, seqs.numel()
+        _check_device(index)
+        _free(self._c, _ints(seqs, "seqs", index, n), n, _on(stream, index))
 
     def compact(self, stream=None):
         """Moves the pages in use to the front of the pool."""
-        _check_device(self.device)
-        _lib.call("oasis_pages_compact", self._ref, _stream(stream))
+        _check_device(self._index)
+        _compact(self._c, _on(stream, self._index))
 
     def check(self):
         """Raises if a call was refused on the device since the last check (synchronizes)."""
@@ -177,31 +213,21 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     sequence. dim is 64 or 128, heads a multiple of kv_heads. Rows of no sequence are
     left as they are in `out`. `longest` (the longest sequence, or a bound) chooses the
     kernel and nothing else."""
-    device = q.device
-    _check_device(device)
-    if q.dim() != 3 or k.dim() != 3:
-        raise ValueError("q, k and v must be [rows, heads, dim]")
-    rows, heads, dim = q.shape
+    index = q.get_device()
+    _check_device(index)
     if q.dtype not in DTYPES:
         raise ValueError(f"q must be bfloat16 or float16, got {q.dtype}")
-    _check_rows(q, "q", q.dtype, device, None, dim)
-    _check_rows(k, "k", q.dtype, device, None, dim)
-    _check_rows(v, "v", q.dtype, device, k.shape[1], dim)
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError(f"q, k and v have {rows}, {k.shape[0]} and {v.shape[0]} rows")
-    _check_ints(cu, "cu", device)
+    dtype, dim = q.dtype, q.shape[-1]
+    rows, heads, q_at, q_row, q_head = _rows(q, "q", dtype, index, None, None, dim)
+    _, kv_heads, k_at, k_row, k_head = _rows(k, "k", dtype, index, rows, None, dim)
+    _, _, v_at, v_row, v_head = _rows(v, "v", dtype, index, rows, kv_heads, dim)
     if out is None:
-        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=device)
-        if stream is not None:
-            out.record_stream(stream)
-    else:
-        _check_rows(out, "out", q.dtype, device, heads, dim)
-        if out.shape[0] != rows:
-            raise ValueError(f"out has {out.shape[0]} rows, q {rows}")
-    a = _lib.OasisPromptArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), *_strides(q), *_strides(k),
-                             *_strides(v), *_strides(out), rows, cu.data_ptr(), max(cu.numel() - 1, 0), longest, heads,
-                             k.shape[1], dim, DTYPES[q.dtype], dim ** -0.5 if scale is None else scale)
-    _lib.call("oasis_attention_prompt", C.byref(a), _stream(stream))
+        out = _new(q, (rows, heads, dim), stream)
+    _, _, out_at, out_row, out_head = _rows(out, "out", dtype, index, rows, heads, dim)
+    n = max(cu.numel() - 1, 0)
+    _prompt(_pack_prompt(q_at, k_at, v_at, out_at, q_row, q_head, k_row, k_head, v_row, v_head, out_row, out_head, rows,
+                         _ints(cu, "cu", index, cu.numel()), n, min(longest, _MOST), heads, kv_heads, dim, DTYPES[dtype],
+                         dim ** -0.5 if scale is None else scale), _on(stream, index))
     return out
 
 
@@ -220,6 +246,7 @@ class SharedPlan:
         self.groups, self.rows = len(group_rows), starts[-1]
         self.group_start = torch.tensor(starts, dtype=torch.int32, device=device)
         self.prefix_pages = torch.tensor(prefix_pages or [0], dtype=torch.int32, device=device)
+        self.bytes = torch.empty(0, dtype=torch.uint8, device=device)  # for workspaces' type and device
         self.longest = longest
         self.most_rows = max(group_rows, default=0)
         self.most_pages = max(prefix_pages, default=0)
@@ -231,33 +258,33 @@ def attention_shared(q: torch.Tensor, cache: PagedCache, layer: int, seqs: torch
     """One query per row: q [rows, heads, head_dim] over the tokens of sequences
     seqs [rows] of the cache, in one layer, after their newest token was written.
     Prefixes that `plan` names are read once for their group."""
-    device = q.device
-    _check_device(device)
-    if cache.device != device or plan.group_start.device != device:
-        raise ValueError(f"q is on {device}, the cache on {cache.device}, the plan on {plan.group_start.device}")
-    _check_rows(q, "q", cache.dtype, device, None, cache.head_dim)
-    rows, heads, dim = q.shape
-    _check_ints(seqs, "seqs", device, rows)
+    index, dim = cache._index, cache.head_dim
+    _check_device(index)
+    if plan.group_start.get_device() != index:
+        raise ValueError(f"the cache is on cuda:{index}, the plan on {plan.group_start.device}")
+    rows, heads, q_at, q_row, q_head = _rows(q, "q", cache.dtype, index, None, None, dim)
+    seqs_at = _ints(seqs, "seqs", index, rows)
     if plan.rows > rows:
         raise ValueError(f"the plan is for {plan.rows} rows, q has {rows}")
     if out is None:
-        out = torch.empty(rows, heads, dim, dtype=q.dtype, device=device)
-        if stream is not None:
-            out.record_stream(stream)
-    else:
-        _check_rows(out, "out", q.dtype, device, heads, dim)
-        if out.shape[0] != rows:
-            raise ValueError(f"out has {out.shape[0]} rows, q {rows}")
-    own = max(0, plan.longest - plan.least_pages * cache.page_size)
-    a = _lib.OasisSharedArgs(q.data_ptr(), out.data_ptr(), *_strides(q), *_strides(out), C.pointer(cache._c), layer,
-                             seqs.data_ptr(), rows, heads, plan.group_start.data_ptr(), plan.prefix_pages.data_ptr(),
-                             plan.groups, plan.most_rows, plan.most_pages, own, dim ** -0.5 if scale is None else scale)
-    ref = C.byref(a)
-    size = _lib.load().oasis_attention_shared_workspace_size(ref)
-    if size:
-        ws = workspace(size, device)
-        if stream is not None:
-            ws.record_stream(stream)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), size
-    _lib.call("oasis_attention_shared", ref, _stream(stream))
+        out = _new(q, (rows, heads, dim), stream)
+    _, _, out_at, out_row, out_head = _rows(out, "out", cache.dtype, index, rows, heads, dim)
+    fields = (q_at, out_at, q_row, q_head, out_row, out_head, cache._at, layer, seqs_at, rows,
+              heads, plan.group_start.data_ptr(), plan.prefix_pages.data_ptr(), plan.groups, plan.most_rows,
+              plan.most_pages, min(max(0, plan.longest - plan.least_pages * cache.page_size), _MOST),
+              dim ** -0.5 if scale is None else scale)
+    size = _shared_workspace(_pack_shared(*fields, 0, 0))
+    ws = _new(plan.bytes, size, stream) if size else None
+    _shared(_pack_shared(*fields, ws.data_ptr() if size else 0, size), _on(stream, index))
     return out
+
+
+def _shared_workspace(args: bytes) -> int:
+    global _size_of
+    if _size_of is None:
+        _size_of = _lib.load()["oasis_attention_shared_workspace_size"]
+        _size_of.restype, _size_of.argtypes = C.c_size_t, (C.c_char_p,)
+    return _size_of(args)
+
+
+_size_of = None
