@@ -399,20 +399,25 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   // an item is a warp's, or a team of four warps takes its units in turn
   const int member = p.team > 1 ? warp : 0;
   long long x = p.team > 1 ? (long long)blockIdx.x : (long long)blockIdx.x * kOwnWarps + warp;
-  const int split = (int)(x % p.own_splits);
-  x /= p.own_splits;
+  // every row's first range comes before the second ones, which few rows may have
   const int ht = (int)(x % p.head_tiles);
   x /= p.head_tiles;
   const int kvh = (int)(x % p.g.kv_heads);
-  const int b = (int)(x / p.g.kv_heads);
-  if (b >= p.rows) {  // whole warps, and whole teams
+  x /= p.g.kv_heads;
+  const int split = (int)(x / p.rows), b = (int)(x % p.rows);
+  if (split >= p.own_splits) {  // whole warps, and whole teams
     pdl_wait();
     return;
   }
-  int s = p.seqs[b];  // on its way during the search
-  const int group = served_group(p, b), P = p.g.page_size;
+  int s = p.seqs[b];
+  const int P = p.g.page_size;
   const bool known = s >= 0 && s < p.g.slots;
   const int len = known ? held_tokens(p.lengths[s], P, p.g.width) : 0;
+  if (split > 0 && (long long)split * p.own_units * kUnit >= len) {  // not even without a prefix
+    pdl_wait();
+    return;
+  }
+  const int group = served_group(p, b);
   const int begin = group_tokens(p, group);
   if (!known) {
     if (lane == 0) atomicOr(p.status, OASIS_PAGES_BAD_SEQUENCE);

@@ -23,7 +23,9 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanPer = 16;       // pages a thread looks at per round of the free-page search
+constexpr int kFewSlots = 8192;    // up to this many sequences, requests' targets are told apart in shared memory
 constexpr int kCopyThreads = 256;
+constexpr int kWriteVectors = 4;   // of 16 bytes, of a thread at a time
 constexpr int kCounters = 16;      // [0] new pages granted, [1] pages moved, [2] live pages
 
 struct PageArgs {
@@ -85,11 +87,21 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PageArgs c, const in
                                                             int n, int deep, int* __restrict__ start) {
   pdl_trigger();
   pdl_wait();
+  __shared__ int few_owners[kFewSlots];
   const int tid = threadIdx.x;
   const int P = c.g.page_size;
-  int *owner = ws_owner(c), *base = ws_base(c), *len = ws_len(c), *list = ws_list(c);
+  int *base = ws_base(c), *len = ws_len(c), *list = ws_list(c);
+  int* owner = c.g.slots <= kFewSlots ? few_owners : ws_owner(c);
   const int* target = FORK ? b : a;
   int bad = 0;
+  auto free_pages = [&](long long p) {  // of the kPlanPer pages from p on, a bit each
+    unsigned mask = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanPer; ++k)
+      if (p + k < c.g.pages && c.refs[p + k] == 0) mask |= 1u << k;
+    return mask;
+  };
+  const unsigned first_free = free_pages((long long)tid * kPlanPer);  // on its way beside the requests
   for (int i = tid; i < n; i += kPlanThreads) {
     const int t = target[i];
     if (t >= 0 && t < c.g.slots) owner[t] = INT_MAX;
@@ -110,7 +122,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PageArgs c, const in
       int keep = -1;  // tokens that the request starts from, -1: refused
       if (t < 0 || t >= c.g.slots) {
         bad |= OASIS_PAGES_BAD_SEQUENCE;
-      } else if (__ldcg(&owner[t]) != i) {
+      } else if (*(volatile int*)&owner[t] != i) {
         bad |= OASIS_PAGES_IN_USE;
       } else if (FORK) {
         const int s = a[i];
@@ -145,10 +157,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PageArgs c, const in
   int found = 0;
   for (long long p0 = 0; p0 < c.g.pages && found < wanted; p0 += kPlanThreads * kPlanPer) {
     const long long p = p0 + (long long)tid * kPlanPer;
-    unsigned free_mask = 0;
-#pragma unroll
-    for (int k = 0; k < kPlanPer; ++k)
-      if (p + k < c.g.pages && c.refs[p + k] == 0) free_mask |= 1u << k;
+    const unsigned free_mask = p0 == 0 ? first_free : free_pages(p);
     int sum;
     int at = found + block_scan(__popc(free_mask), &sum);
 #pragma unroll
@@ -227,10 +236,19 @@ __device__ __forceinline__ void copy_page(const PageArgs& c, int from, int to, i
   }
 }
 
+// Parts that each of `pages` pages' copies is cut into, so that every block of the grid
+// has a part, or several where there are many pages. A unit begins with a chain of
+// lookups (request, sequence, table), so there should be few of them.
+__device__ __forceinline__ int copy_parts(const PageArgs& c, int pages) {
+  const long long want = pages > 0 ? (gridDim.x + pages - 1LL) / pages : 1, most = page_vectors(c.g) / kCopyThreads;
+  const long long parts = want < 4 ? 4 : want;
+  return (int)(parts < most ? parts : most < 1 ? 1 : most);
+}
+
 // After plan_kernel<true>: the targets' table rows, the shared pages' counts and
 // the copies. Sources are not targets of the same call unless they were empty.
 __global__ void __launch_bounds__(kCopyThreads) fork_kernel(PageArgs c, const int* __restrict__ src,
-                                                            const int* __restrict__ dst, int n, int deep, int parts) {
+                                                            const int* __restrict__ dst, int n, int deep) {
   pdl_trigger();
   pdl_wait();
   const int P = c.g.page_size, W = c.g.width;
@@ -255,6 +273,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(PageArgs c, const in
       to[k] = page;
     }
   }
+  const int parts = copy_parts(c, c.ws[0]);
   const long long units = (long long)c.ws[0] * parts;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
     const int k = (int)(u / parts);
@@ -333,7 +352,7 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(PageArgs c) 
   }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) compact_kernel(PageArgs c, int parts) {
+__global__ void __launch_bounds__(kCopyThreads) compact_kernel(PageArgs c) {
   pdl_trigger();
   pdl_wait();
   const int moves = c.ws[1], live = c.ws[2];
@@ -352,6 +371,7 @@ __global__ void __launch_bounds__(kCopyThreads) compact_kernel(PageArgs c, int p
       }
     }
   }
+  const int parts = copy_parts(c, moves);
   const long long units = (long long)moves * parts;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
     const int k = (int)(u / parts);
@@ -359,8 +379,12 @@ __global__ void __launch_bounds__(kCopyThreads) compact_kernel(PageArgs c, int p
   }
 }
 
-// New key and value rows of one layer into their pages: a 16-byte vector per thread,
+// New key and value rows of one layer into their pages: four 16-byte vectors per thread,
+// loaded before the chain of lookups that says where they go (9 us a layer of 18 MB with
+// the loads behind it and one vector per thread),
 // row r of the packed rows at position start[i] + r - cu[i] of sequence seqs[i].
+// V: 1 where that many threads still fit the GPU at once, else kWriteVectors.
+template <int V>
 __global__ void __launch_bounds__(kCopyThreads) write_kernel(PageArgs c, int layer, const uint4* __restrict__ k,
                                                              const uint4* __restrict__ v, long long k_row,
                                                              long long k_head, long long v_row, long long v_head,
@@ -371,11 +395,24 @@ __global__ void __launch_bounds__(kCopyThreads) write_kernel(PageArgs c, int lay
   const int rv = row_vectors(c.g), K = c.g.kv_heads;
   const unsigned per = (unsigned)(2 * K * rv);
   const int last = min(rows, cu[n]);
-  const long long all = (long long)last * per;
-  for (long long x = (long long)blockIdx.x * kCopyThreads + threadIdx.x; x < all;
-       x += (long long)gridDim.x * kCopyThreads) {
-    const int r = (int)(x / per);
-    const unsigned w = (unsigned)(x - (long long)r * per);
+  // `width` threads to a row, so `group` rows at a time; longer rows in several rounds
+  const unsigned width = min((per + V - 1) / V, (unsigned)kCopyThreads), group = kCopyThreads / width;
+  const unsigned in_row = threadIdx.x % width, first = threadIdx.x / width;
+  if (first >= group) return;
+  for (long long r0 = (long long)blockIdx.x * group + first; r0 < last; r0 += (long long)gridDim.x * group) {
+    const int r = (int)r0;
+    const uint4 *k_at = k + r * k_row, *v_at = v + r * v_row;
+    uint4 data[V];
+    auto fetch = [&](unsigned w0) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const unsigned w = w0 + j * width;
+        if (w >= per) continue;
+        const unsigned tile_row = w / rv, d = w - tile_row * rv;  // (keys or values, head)
+        data[j] = tile_row >= (unsigned)K ? v_at[(tile_row - K) * v_head + d] : k_at[tile_row * k_head + d];
+      }
+    };
+    fetch(in_row);
     const int i = last_not_above(cu, n, r);
     const int s = seqs[i], begin = start[i];
     if (begin < 0 || s < 0 || s >= c.g.slots) continue;
@@ -387,11 +424,18 @@ __global__ void __launch_bounds__(kCopyThreads) write_kernel(PageArgs c, int lay
       atomicOr(c.status, OASIS_PAGES_BAD_PAGE);
       continue;
     }
-    const int which = w >= per / 2;
-    const unsigned y = w - which * (per / 2);
-    const int head = y / rv, d = y - head * rv;
-    const uint4 data = which ? v[r * v_row + head * v_head + d] : k[r * k_row + head * k_head + d];
-    c.pool[tile_offset(c.g, page, layer, which, head) + (long long)slot * rv + d] = data;
+    uint4* to = c.pool + tile_offset(c.g, page, layer, 0, 0) + (long long)slot * rv;
+    const long long tile = tile_vectors(c.g);
+    for (unsigned w0 = in_row; w0 < per; w0 += V * width) {
+      if (w0 != in_row) fetch(w0);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const unsigned w = w0 + j * width;
+        if (w >= per) continue;
+        const unsigned tile_row = w / rv, d = w - tile_row * rv;
+        to[tile_row * tile + d] = data[j];
+      }
+    }
   }
 }
 
@@ -435,8 +479,8 @@ int check_cache(const OasisPageCache* c, PageArgs* p, const char* what, bool pla
   return OASIS_OK;
 }
 
-// Blocks that share one page's copy: about 16 KB each, so that a few pages fill the GPU.
-int copy_parts(const PageGeometry& g) {
+// Blocks that one page's copy can keep busy.
+int page_parts(const PageGeometry& g) {
   const long long parts = page_vectors(g) / (4 * kCopyThreads);
   return (int)(parts < 1 ? 1 : parts > 64 ? 64 : parts);
 }
@@ -493,9 +537,11 @@ int oasis_pages_write(const OasisPageCache* cache, int layer, const void* k, con
   OASIS_REQUIRE(((k_row_stride | k_head_stride | v_row_stride | v_head_stride) & 7) == 0,
                 "pages_write: strides %lld %lld %lld %lld are not multiples of 8 elements", k_row_stride, k_head_stride,
                 v_row_stride, v_head_stride);
-  const long long blocks = ((long long)rows * 2 * p.g.kv_heads * row_vectors(p.g) + kCopyThreads - 1) / kCopyThreads;
+  const long long per = 2LL * p.g.kv_heads * row_vectors(p.g), each = per * rows > 4LL * kCopyThreads * num_sms() ? kWriteVectors : 1;
+  const long long width = (per + each - 1) / each, group = width < kCopyThreads ? kCopyThreads / width : 1;  // rows of a block
+  const long long blocks = (rows + group - 1) / group;
   const long long most = 16LL * num_sms();
-  return launched(launch_pdl(write_kernel, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kCopyThreads), 0,
+  return launched(launch_pdl(each == 1 ? write_kernel<1> : write_kernel<kWriteVectors>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(kCopyThreads), 0,
                              static_cast<cudaStream_t>(stream), p, layer, static_cast<const uint4*>(k),
                              static_cast<const uint4*>(v), k_row_stride / 8, k_head_stride / 8, v_row_stride / 8,
                              v_head_stride / 8, seqs, cu, start, n, rows),
@@ -513,10 +559,8 @@ int oasis_pages_fork(const OasisPageCache* cache, const int* src, const int* dst
   OASIS_TRY(launched(launch_pdl(plan_kernel<true>, dim3(1), dim3(kPlanThreads), 0, st, p, src, dst,
                                 static_cast<const int*>(nullptr), n, deep ? 1 : 0, static_cast<int*>(nullptr)),
                      "pages_fork (plan)"));
-  const int parts = copy_parts(p.g);
-  return launched(launch_pdl(fork_kernel, dim3(copy_blocks((long long)n * (deep ? p.g.width : 1) * parts)),
-                             dim3(kCopyThreads), 0, st, p, src, dst, n,
-                             deep ? 1 : 0, parts),
+  return launched(launch_pdl(fork_kernel, dim3(copy_blocks((long long)n * (deep ? p.g.width : 1) * page_parts(p.g))),
+                             dim3(kCopyThreads), 0, st, p, src, dst, n, deep ? 1 : 0),
                   "pages_fork");
 }
 
@@ -535,9 +579,8 @@ int oasis_pages_compact(const OasisPageCache* cache, oasis_stream_t stream) {
   OASIS_TRY(check_cache(cache, &p, "pages_compact", true));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   OASIS_TRY(launched(launch_pdl(compact_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, p), "pages_compact (plan)"));
-  const int parts = copy_parts(p.g);
-  return launched(launch_pdl(compact_kernel, dim3(copy_blocks((long long)(p.g.pages / 2 + 1) * parts)),
-                             dim3(kCopyThreads), 0, st, p, parts),
+  return launched(launch_pdl(compact_kernel, dim3(copy_blocks((long long)(p.g.pages / 2 + 1) * page_parts(p.g))),
+                             dim3(kCopyThreads), 0, st, p),
                   "pages_compact");
 }
 

@@ -265,11 +265,14 @@ def test_random_runs(seed, pages, slots):
 
 
 @pytest.mark.gpu
-def test_many_requests_at_once():
-    """More requests than the planning block has threads."""
-    c, o = make(pages=4000, page=16, layers=1, heads=1, dim=8, slots=2500, width=3)
+@pytest.mark.parametrize("slots", [2500, 9000])
+def test_many_requests_at_once(slots):
+    """More requests than the planning block has threads; more sequences than it keeps in
+    shared memory."""
+    c, o = make(pages=4000, page=16, layers=1, heads=1, dim=8, slots=slots, width=3)
     rng = random.Random(5)
-    seqs = list(range(2500))
+    seqs = rng.sample(range(slots), 2499)
+    seqs.insert(1300, seqs[7])  # named twice
     rng.shuffle(seqs)
     counts = [rng.choice([0, 1, 16, 17, 48, 49]) for _ in seqs]
     cu = [0]
