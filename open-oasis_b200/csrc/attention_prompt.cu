@@ -59,18 +59,30 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
 
   uint8_t* const sk = sm + Q_BYTES;
   uint8_t* const sv = sk + K_BYTES;
-  for (int x = tid; x < kRowsTile * CH; x += kRowsThreads) {
-    const int r = x / CH, c = x % CH;
-    const bool ok = r0 + r < p.rows;
-    cp_async16(sm + tile_at<D>(r, c), q + (ok ? r0 + r : 0) * p.q_row + c * 8, ok);
+  // A thread's 16-byte chunks lie STEP rows apart, in the same swizzled column.
+  constexpr int STEP = kRowsThreads / CH;
+  static_assert(STEP % 8 == 0 && kRowsTile % STEP == 0 && kRowsKeys % STEP == 0, "chunks of a thread");
+  const int tr = tid / CH, tc = tid % CH;
+  {
+    const T* from = q + (long long)(r0 + tr) * p.q_row + tc * 8;
+    uint8_t* to = sm + tile_at<D>(tr, tc);
+#pragma unroll
+    for (int i = 0; i < kRowsTile / STEP; ++i) {
+      const bool ok = r0 + tr + i * STEP < p.rows;
+      cp_async16(to + i * STEP * D * 2, ok ? from : q, ok);
+      from += STEP * p.q_row;
+    }
   }
   auto load = [&](int at) {
-    for (int x = tid; x < kRowsKeys * CH; x += kRowsThreads) {
-      const int r = x / CH, c = x % CH;
-      const bool ok = at + r >= 0 && at + r < p.rows;
-      const long long row = ok ? at + r : 0;
-      cp_async16(sk + tile_at<D>(r, c), k + row * p.k_row + c * 8, ok);
-      cp_async16(sv + tile_at<D>(r, c), v + row * p.v_row + c * 8, ok);
+    const T *k_from = k + (long long)(at + tr) * p.k_row + tc * 8, *v_from = v + (long long)(at + tr) * p.v_row + tc * 8;
+    uint8_t* to = sk + tile_at<D>(tr, tc);
+#pragma unroll
+    for (int i = 0; i < kRowsKeys / STEP; ++i) {
+      const bool ok = (unsigned)(at + tr + i * STEP) < (unsigned)p.rows;
+      cp_async16(to + i * STEP * D * 2, ok ? k_from : k, ok);
+      cp_async16(to + K_BYTES + i * STEP * D * 2, ok ? v_from : v, ok);
+      k_from += STEP * p.k_row;
+      v_from += STEP * p.v_row;
     }
   };
   load(r0 - kRowsBefore);
@@ -112,6 +124,9 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
   const int wr = warp * 16;  // this warp's first row in the tile
   const int ra = wr + (lane >> 2), rb = ra + 8;
   const int lo_a = first[ra], lo_b = first[rb];
+  // keys lo .. lo + span are seen; a row of nobody sees none, its lo lies behind all keys
+  const unsigned span_a = lo_a <= r0 + ra ? r0 + ra - lo_a : 0, span_b = lo_b <= r0 + rb ? r0 + rb - lo_b : 0;
+  const int from_a = lo_a <= r0 + ra ? lo_a : 0x3fffffff, from_b = lo_b <= r0 + rb ? lo_b : 0x3fffffff;
   const int low = __reduce_min_sync(0xffffffffu, min(lo_a, lo_b)), high = __reduce_max_sync(0xffffffffu, max(lo_a, lo_b));
   uint32_t qa[KS][4];
   float o[NT][4];
@@ -144,16 +159,16 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
         E::mma(x[1], qa[s], b[2], b[3]);
       }
       const bool whole = kb >= high && kb + 15 <= r0 + wr;
+      if (!whole) {
+        const int key = kb + (lane & 3) * 2;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+        for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = kb + t * 8 + (lane & 3) * 2 + (e & 1);
-          const bool see = whole || (e < 2 ? key >= lo_a && key <= r0 + ra : key >= lo_b && key <= r0 + rb);
-          x[t][e] = see ? x[t][e] * p.scale_log2 : -INFINITY;
-        }
-      float na = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1]));
-      float nb = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3]));
+          for (int e = 0; e < 4; ++e)
+            if ((unsigned)(key - (e < 2 ? from_a : from_b) + t * 8 + (e & 1)) > (e < 2 ? span_a : span_b)) x[t][e] = -INFINITY;
+      }
+      float na = fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[1][0], x[1][1])) * p.scale_log2;
+      float nb = fmaxf(fmaxf(x[0][2], x[0][3]), fmaxf(x[1][2], x[1][3])) * p.scale_log2;
 #pragma unroll
       for (int w = 1; w < 4; w <<= 1) {
         na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, w));
@@ -167,10 +182,10 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
       mb = nb;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        x[t][0] = ex2_approx(x[t][0] - sa);
-        x[t][1] = ex2_approx(x[t][1] - sa);
-        x[t][2] = ex2_approx(x[t][2] - sb);
-        x[t][3] = ex2_approx(x[t][3] - sb);
+        x[t][0] = ex2_approx(fmaf(x[t][0], p.scale_log2, -sa));
+        x[t][1] = ex2_approx(fmaf(x[t][1], p.scale_log2, -sa));
+        x[t][2] = ex2_approx(fmaf(x[t][2], p.scale_log2, -sb));
+        x[t][3] = ex2_approx(fmaf(x[t][3], p.scale_log2, -sb));
       }
       la = la * fa + ((x[0][0] + x[0][1]) + (x[1][0] + x[1][1]));  // this lane's share; joined at the end
       lb = lb * fb + ((x[0][2] + x[0][3]) + (x[1][2] + x[1][3]));
@@ -211,12 +226,12 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
   const unsigned bad_a = __ballot_sync(0xffffffffu, !ok_a), bad_b = __ballot_sync(0xffffffffu, !ok_b);
   __syncwarp();
   T* out = static_cast<T*>(p.out) + head * p.o_head;
+  T* to = out + (long long)(r0 + wr + lane / CH) * p.o_row + lane % CH * 8;
 #pragma unroll
-  for (int x = lane; x < 16 * CH; x += 32) {
-    const int r = x / CH, c = x % CH;
-    const int row = r0 + wr + r;
-    if (first[wr + r] <= row)
-      *reinterpret_cast<uint4*>(out + row * p.o_row + c * 8) = *reinterpret_cast<const uint4*>(sm + tile_at<D>(wr + r, c));
+  for (int i = 0; i < 16 * CH / 32; ++i) {
+    const int r = wr + i * (32 / CH) + lane / CH;
+    if (first[r] <= r0 + r) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(sm + tile_at<D>(r, lane % CH));
+    to += (32 / CH) * p.o_row;
   }
   if ((bad_a | bad_b) == 0) return;
   __syncwarp();
