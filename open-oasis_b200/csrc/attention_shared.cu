@@ -323,11 +323,11 @@ __device__ __forceinline__ void column_step(Columns<D>& c, const uint8_t* sk, co
     Elem<T>::mma(x, a, qb[s][0], qb[s][1]);
   }
   const int key = key0 + (lane >> 2);
-  x[0] = key < lim_a ? x[0] * scale_log2 : -INFINITY;
-  x[1] = key < lim_b ? x[1] * scale_log2 : -INFINITY;
-  x[2] = key + 8 < lim_a ? x[2] * scale_log2 : -INFINITY;
-  x[3] = key + 8 < lim_b ? x[3] * scale_log2 : -INFINITY;
-  float na = fmaxf(x[0], x[2]), nb = fmaxf(x[1], x[3]);
+  if (key >= lim_a) x[0] = -INFINITY;
+  if (key >= lim_b) x[1] = -INFINITY;
+  if (key + 8 >= lim_a) x[2] = -INFINITY;
+  if (key + 8 >= lim_b) x[3] = -INFINITY;
+  float na = fmaxf(x[0], x[2]) * scale_log2, nb = fmaxf(x[1], x[3]) * scale_log2;
 #pragma unroll
   for (int w = 4; w < 32; w <<= 1) {
     na = fmaxf(na, __shfl_xor_sync(0xffffffffu, na, w));
@@ -339,10 +339,10 @@ __device__ __forceinline__ void column_step(Columns<D>& c, const uint8_t* sk, co
   const float fa = ex2_approx(c.m[0] - sa), fb = ex2_approx(c.m[1] - sb);
   c.m[0] = na;
   c.m[1] = nb;
-  x[0] = ex2_approx(x[0] - sa);
-  x[1] = ex2_approx(x[1] - sb);
-  x[2] = ex2_approx(x[2] - sa);
-  x[3] = ex2_approx(x[3] - sb);
+  x[0] = ex2_approx(fmaf(x[0], scale_log2, -sa));
+  x[1] = ex2_approx(fmaf(x[1], scale_log2, -sb));
+  x[2] = ex2_approx(fmaf(x[2], scale_log2, -sa));
+  x[3] = ex2_approx(fmaf(x[3], scale_log2, -sb));
   c.l[0] = c.l[0] * fa + (x[0] + x[2]);
   c.l[1] = c.l[1] * fb + (x[1] + x[3]);
   // P^T (keys x queries) turned into the second operand: the one rounding inside the sum
