@@ -111,7 +111,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   using C = Cfg<D>;
   using E = Elem<T>;
   extern __shared__ uint8_t smem_raw[];
-  pdl_trigger();
   pdl_wait();
   const int end = min(p.rows, p.cu[p.n]);
   // Work: a row tile (pair) x a head (pair), the last rows first: in a sequence those
@@ -153,8 +152,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
     fence_barrier_init();
   }
   if (warp == 9) {
+    // What follows starts early only once this block has its TMEM: a kernel that took some
+    // of it first and then waited for this grid would never get to give it back.
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
+    pdl_trigger();
   }
   tc_fence_before();
   __syncthreads();

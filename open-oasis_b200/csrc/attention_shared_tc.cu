@@ -49,7 +49,6 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
   using E = Elem<T>;
   extern __shared__ uint8_t smem_raw[];
   pdl_wait();
-  pdl_trigger();  // behind the wait: the kernel of the own keys starts without one
   int x = blockIdx.x;
   const int pair = x % p.tiles;
   x /= p.tiles;
@@ -97,8 +96,12 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
     fence_barrier_init();
   }
   if (warp == 9) {
+    // The trigger is behind the wait, since the kernel of the own keys starts without one,
+    // and behind the allocation: a kernel that took TMEM first and then waited for this
+    // grid would never get to give it back.
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
+    pdl_trigger();
   }
   // The prefix is read through the table row of the longest sequence (the first of
   // them): a shorter one need not have all of its pages.

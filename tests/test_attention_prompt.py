@@ -269,6 +269,39 @@ def test_same_results_again_and_in_a_graph():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+def test_beside_matrix_products(dim):
+    """Products that use tensor memory before and behind the attention, without a pause:
+    each starts while the one before it still runs."""
+    lengths, heads = [150, 90, 16], 8
+    q, k, v = inputs(lengths, heads, 4, dim, BF16, seed=15)
+    cu, rows, width = ints(starts(lengths)), sum(lengths), heads * dim
+    w = (torch.randn(1024, width, device=DEV) * 0.05).to(BF16)
+    big = torch.randn(4096, width, device=DEV).to(BF16)
+    y, z = torch.empty(rows, 1024, device=DEV), torch.empty(4096, 1024, device=DEV)
+    ws = torch.empty(64 << 20, dtype=torch.uint8, device=DEV)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def product(a, out, block_n):
+        args = _lib.OasisGemmArgs()
+        args.a, args.lda, args.w = a.data_ptr(), width, w.data_ptr()
+        args.m, args.n, args.k, args.mode = a.shape[0], 1024, width, 0
+        args.out, args.ldo, args.rows_per_frame, args.rope_div, args.rope_mod = out.data_ptr(), 1024, 1, 1, 1
+        args.block_n, args.splits, args.workspace, args.workspace_bytes = block_n, 1, ws.data_ptr(), ws.numel()
+        _lib.call("oasis_gemm", C.byref(args), stream)
+
+    for block_n in (32, 64, 256):
+        for _ in range(20):
+            product(big, z, block_n)
+            out = paged.attention_prompt(q, k, v, cu, 1 << 20)
+            product(out, y, block_n)
+        check(out, q, k, v, starts(lengths))
+        want = out.reshape(rows, width).double() @ w.double().T
+        assert float((y.double() - want).norm() / want.norm()) < 1e-5
+    assert _lib.load().oasis_device_error(0) == 0
+
+
+@pytest.mark.gpu
 def test_against_the_temporal_attention():
     """One length for all sequences and 16 heads of 64: what oasis_attention_temporal computes."""
     B, T, P = 3, 8, 144
