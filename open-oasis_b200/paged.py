@@ -92,10 +92,14 @@ def _rows(t: torch.Tensor, name: str, dtype, index: int, rows: int | None, heads
 
 
 def _new(t: torch.Tensor, shape, stream) -> torch.Tensor:
-    """An output of a call on `stream`."""
-    out = t.new_empty(shape)
-    if stream is not None:
-        out.record_stream(stream)
+    """An output or a workspace of a call on `stream`: memory that this stream's earlier work
+    has left (the current stream may still use what it gave back), kept from it until
+    what the current stream does with the result is done."""
+    if stream is None:
+        return t.new_empty(shape)
+    with torch.cuda.stream(stream):
+        out = t.new_empty(shape)
+    out.record_stream(torch.cuda.current_stream())
     return out
 
 
@@ -199,7 +203,8 @@ class PagedCache:
         _compact(self._c, _on(stream, self._index))
 
     def check(self):
-        """Raises if a call was refused on the device since the last check (synchronizes)."""
+        """Raises if a call was refused on the device since the last check (synchronizes;
+        a call on the current stream, ordered like the others)."""
         bits = int(self.status.item())
         if bits:
             self.status.zero_()

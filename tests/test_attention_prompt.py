@@ -269,6 +269,30 @@ def test_same_results_again_and_in_a_graph():
 
 
 @pytest.mark.gpu
+def test_memory_of_a_side_stream_is_its_own():
+    """A result on a side stream does not land in memory that the current stream has given
+    back but still reads, and is not given to that side stream again while the current
+    one reads it."""
+    q, k, v = inputs([100], 16, 16, 64, BF16, seed=16)
+    cu, side, zero = ints([0, 100]), torch.cuda.Stream(), torch.zeros(100, 16, 64, dtype=BF16, device=DEV)
+    want = paged.attention_prompt(q, k, v, cu, 100)
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        old = torch.full_like(want, 3.0)
+        torch.cuda._sleep(20_000_000)  # the current stream is busy for some milliseconds
+        kept = old.clone()
+        del old
+        out = paged.attention_prompt(q, k, v, cu, 100, stream=side)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(20_000_000)
+        again = out.clone()
+        del out
+        paged.attention_prompt(q, k, zero, cu, 100, stream=side)
+        torch.cuda.synchronize()
+        assert bool((kept == 3).all()) and torch.equal(again, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128])
 def test_beside_matrix_products(dim):
     """Products that use tensor memory before and behind the attention, without a pause:
