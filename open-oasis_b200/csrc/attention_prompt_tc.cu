@@ -38,10 +38,7 @@ namespace {
 constexpr int kPromptThreads = 384;
 // Of every eight pairs of exponentials this many go to the FMA pipe, the others to the
 // special-function unit, which alone would be the bound.
-#ifndef OASIS_PROMPT_POLY
-#define OASIS_PROMPT_POLY 2
-#endif
-constexpr int kPoly = OASIS_PROMPT_POLY;
+constexpr int kPoly = 2;
 
 template <int D>
 struct Cfg {

@@ -25,11 +25,14 @@ constexpr int kPrefixKeys = 64;     // keys of a step
 constexpr int kWholeRows = 32;      // queries of a block of the one-pass kernel
 constexpr int kThreads = 128;
 constexpr int kOwnWarps = 4;
-// Prefixes of at least this many tokens run on the tensor-memory kernel.
-#ifndef OASIS_TENSOR_KEYS
-#define OASIS_TENSOR_KEYS 256
-#endif
-constexpr int kTensorKeys = OASIS_TENSOR_KEYS;
+// Prefixes of at least this many tokens run on the tensor-memory kernel. Where each of its
+// blocks has at most 64 of its 256 queries and they come in several waves (an SM holds
+// one), it is one token more for each block behind the first wave, up to the second number. Tensor memory / mma.sync, us, own keys included: 8 groups of up to
+// 128 rows, 16 heads of 64: 46.7 / 46.0 for up to 128 tokens, 47.3 / 48.1 for 256, 61.5 / 90.9
+// for 2048; 32 / 8 heads of 128: 49.7 / 47.8, 51.8 / 56.7, 77 / 182. 36 groups of up to 16
+// rows, 16 heads of 64: 60.4 / 41.5 for 256, 63.3 / 53.0 for 512, 77 / 121 for 2048; 20 groups
+// of up to 8 rows: 39.3 / 42.7 for 500.
+constexpr int kTensorKeys = 256, kTensorKeysMost = 700;
 constexpr int kMostSplits = 64;    // of a prefix, and of a row's own keys
 constexpr int kMostRanges = 2 * kMostSplits;
 
@@ -966,7 +969,9 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   if (prefix) {
     const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
     const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
-    p->tensor = keys >= kTensorKeys && pool_rows < (1LL << 31);
+    long long least = kTensorKeys;
+    if (p->tiles == 1 && (long long)a->groups * K > sms) least += (long long)a->groups * K - sms;
+    p->tensor = keys >= (least < kTensorKeysMost ? least : kTensorKeysMost) && pool_rows < (1LL << 31);
     if (p->tensor) {
       // one block for each SM, and at least 128 keys for each block
       const long long pairs = ((long long)group_rows * p->per + 255) / 256;
@@ -986,16 +991,22 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   }
   // A row's own keys go to teams of four warps in ranges of one length, so that a row
   // longer than the others only has more of them: at least 256 keys, as many ranges as
-  // make 12 teams for each SM where all rows have the hinted length. Up to 32 keys are
-  // one warp's.
+  // make 12 teams for each SM where all rows have the hinted length. Where that length is
+  // small for the number of items (row, key head, eight heads), an item is one warp's: a
+  // block's lookups and its end then serve four items, and the longest row's warp takes
+  // four times as long. One warp / four, us, ragged rows in groups, so many items with rows
+  // of up to so many tokens behind their prefix: heads of 64: 272 items 12.6 / 13.6 (64), 20.5 /
+  // 13.8 (256); 2512 items 19.5 / 28.8 (64), 30.4 / 32.6 (256), 80 / 47 (1024); 12544 items 47 /
+  // 109 (64), 138 / 159 (1024). Heads of 128, where an SM holds half as many blocks: 536
+  // items 18.9 / 23.1 (64), 24.1 / 25.2 (256), 83 / 54 (4096); 6272 items 56 / 117 (64), 138 / 165 (1024).
   const long long items = (long long)a->rows * K * p->head_tiles;
   const long long own = a->own_tokens_hint;
-  long long n = (12LL * sms + items - 1) / items;
-  if (n > kMostSplits) n = kMostSplits;
   const long long units = (own + kUnit - 1) / kUnit;
+  p->team = units <= 8 + items * a->cache->head_dim / 8192 ? 1 : kOwnWarps;
+  long long n = p->team == 1 ? 1 : (12LL * sms + items - 1) / items;
+  if (n > kMostSplits) n = kMostSplits;
   long long each = (units + n - 1) / n;
   if (each < 16) each = 16;
-  p->team = units > 2 ? kOwnWarps : 1;
   p->own_units = (int)each;
   p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
   // One pass where its blocks fill the GPU and a warp has at most 32 steps of own keys
