@@ -636,7 +636,8 @@ int oasis_attention_prompt(const OasisPromptArgs* a, oasis_stream_t stream);
  * hints (largest group, longest prefix, most tokens behind a prefix) choose tiles and
  * splits and nothing else; prefix_pages_hint = 0 shares nothing. The call's workspace
  * is oasis_attention_shared_workspace_size(args) bytes (0: none) and must not be used
- * by a call that may run at the same time. Stands beside
+ * by a call that may run at the same time. The output must not overlap q or the
+ * cache. Stands beside
  * oasis_attention_temporal_cached (one context length for all, no sharing). */
 typedef struct OasisSharedArgs {
   const void* q; void* out;

@@ -6,11 +6,20 @@
 // o = sum e^(m_r - m) o~_r / l.
 //
 // shared_prefix_kernel: the keys that a group's rows have in common, read once for all
-// of them: 64 (row, head) queries of one key head per block, 64 keys a step, mma.sync.
+// of them: 64 (row, head) queries of one key head per block, 64 keys a step, mma.sync; for
+// short prefixes (attention_shared_tc.cu has the others). Bound by latency: a block of few
+// steps loads its rows' lengths, the table and the keys one behind the other.
 // shared_own_kernel: each row's keys behind the prefix: four warps (or one) per (row, key
 // head, range), 16 keys a step, the heads of a key head as the eight columns of a fragment.
-// Bound by reading the keys and values once. With one split it joins the prefix ranges too and
-// writes the result; otherwise shared_join_kernel does.
+// The least is reading the keys and values once: 32 rows of up to 4096 tokens, 32 / 8 heads
+// of 128, 97 MB: 38 us (2.5 TB/s) with the join; a block's lookups before its first load,
+// two steps of keys in flight per warp and the rows' different lengths are the rest. It
+// runs beside the prefix kernel. With one range it joins the prefix's and
+// writes the result; otherwise shared_join_kernel does, a warp per (row, head).
+// 64 rows behind 8192 shared tokens, up to 1024 own ones, 32 / 8 heads of 128: 51 us, about
+// 25 for the prefix, 23 for the own keys beside and behind it and 10 for the join; the
+// bytes alone would take 10.
+// shared_whole_kernel: both in one pass where rows are many and short.
 #include "../../include/oasis_b200.h"
 #include "attention_rows.cuh"
 #include "attention_shared.cuh"
@@ -27,11 +36,12 @@ constexpr int kThreads = 128;
 constexpr int kOwnWarps = 4;
 // Prefixes of at least this many tokens run on the tensor-memory kernel. Where each of its
 // blocks has at most 64 of its 256 queries and they come in several waves (an SM holds
-// one), it is one token more for each block behind the first wave, up to the second number. Tensor memory / mma.sync, us, own keys included: 8 groups of up to
-// 128 rows, 16 heads of 64: 46.7 / 46.0 for up to 128 tokens, 47.3 / 48.1 for 256, 61.5 / 90.9
-// for 2048; 32 / 8 heads of 128: 49.7 / 47.8, 51.8 / 56.7, 77 / 182. 36 groups of up to 16
-// rows, 16 heads of 64: 60.4 / 41.5 for 256, 63.3 / 53.0 for 512, 77 / 121 for 2048; 20 groups
-// of up to 8 rows: 39.3 / 42.7 for 500.
+// one), it is one token more for each block behind the first wave, up to the second
+// number. Tensor memory / mma.sync, us, own keys included: 8 groups of up to 128 rows, 16
+// heads of 64: 46.7 / 46.0 for up to 128 tokens, 47.3 / 48.1 for 256, 61.5 / 90.9 for 2048;
+// 32 / 8 heads of 128: 49.7 / 47.8, 51.8 / 56.7, 77 / 182. 36 groups of up to 16 rows, 16
+// heads of 64: 60.4 / 41.5 for 256, 63.3 / 53.0 for 512, 77 / 121 for 2048; 20 groups of up to
+// 8 rows: 39.3 / 42.7 for 500.
 constexpr int kTensorKeys = 256, kTensorKeysMost = 700;
 constexpr int kMostSplits = 64;    // of a prefix, and of a row's own keys
 constexpr int kMostRanges = 2 * kMostSplits;
@@ -609,6 +619,9 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
 // a row's first 16 keys find its O empty and need no rescaling. Then each
 // group's prefix is read once for the rows of the tile that are in it. Bound by issue:
 // about 200 instructions for each row's 16 keys, and by the latency of their loads.
+// 9216 rows in 144 groups, 16 + up to 16 tokens each, 16 heads of 64, 255 MB: 108 us (2.4
+// TB/s; one warp per row and head in two kernels 124 us). 64 queries and 8 warps a block,
+// for groups of 16 rows: 35 -> 45 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, D == 64 ? 6 : 3) shared_whole_kernel(SharedParams p) {
   constexpr int CH = D / 8, KS = D / 16, MT = D / 16, TILE = kPrefixKeys * D * 2, UNIT = kUnit * D * 2;

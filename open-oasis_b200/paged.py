@@ -216,8 +216,8 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
     """Causal attention within packed sequences: rows [cu[i], cu[i + 1]) of q [rows, heads,
     dim] and k, v [rows, kv_heads, dim] (views of packed QKV rows are fine) are one
     sequence. dim is 64 or 128, heads a multiple of kv_heads. Rows of no sequence are
-    left as they are in `out`. `longest` (the longest sequence, or a bound) chooses the
-    kernel and nothing else."""
+    left as they are in `out`, which must not overlap q, k or v. `longest` (the longest
+    sequence, or a bound) chooses the kernel and nothing else."""
     index = q.get_device()
     _check_device(index)
     if q.dtype not in DTYPES:
@@ -262,7 +262,8 @@ def attention_shared(q: torch.Tensor, cache: PagedCache, layer: int, seqs: torch
                      out: torch.Tensor | None = None, scale: float | None = None, stream=None) -> torch.Tensor:
     """One query per row: q [rows, heads, head_dim] over the tokens of sequences
     seqs [rows] of the cache, in one layer, after their newest token was written.
-    Prefixes that `plan` names are read once for their group."""
+    Prefixes that `plan` names are read once for their group. `out` must not overlap q
+    or the cache."""
     index, dim = cache._index, cache.head_dim
     _check_device(index)
     if plan.group_start.get_device() != index:
