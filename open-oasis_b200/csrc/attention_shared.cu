@@ -571,20 +571,31 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   for (int half = 0; half < 2; ++half) {
     const bool mine = ca + half < nh;
     const long long slot = ((long long)b * p.heads + h0 + (mine ? ca + half : 0)) * splits;
-    float m = run.m[half], l = run.l[half];
+    const float m = run.m[half];
+    float l = run.l[half];
     if (group >= 0 && mine) {
+      // the joint maximum first, so that the ranges' loads do not wait for one another
+      float top = m;
+#pragma unroll 4
+      for (int i = 0; i < p.prefix_splits; ++i) top = fmaxf(top, p.part_ml[slot + i].x);
+      const float sh = softmax_shift(top), fo = ex2_approx(m - sh);
+      l *= fo;
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        run.o[t][half] *= fo;
+        run.o[t][half + 2] *= fo;
+      }
+#pragma unroll 4
       for (int i = 0; i < p.prefix_splits; ++i) {
         const float2 ml = p.part_ml[slot + i];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float n = fmaxf(m, ml.x), sh = softmax_shift(n);
-        const float fo = ex2_approx(m - sh), fp = ex2_approx(ml.x - sh);
-        l = l * fo + ml.y * fp;
-        m = n;
+        const float f = ex2_approx(ml.x - sh);
+        l = fmaf(ml.y, f, l);
+        const bool some = !(ml.x == -INFINITY && ml.y == 0.f);  // its sums were written
         const float* y = p.part_o + (slot + i) * D + dim;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-          run.o[t][half] = run.o[t][half] * fo + y[t * 16] * fp;
-          run.o[t][half + 2] = run.o[t][half + 2] * fo + y[t * 16 + 8] * fp;
+          run.o[t][half] = fmaf(some ? y[t * 16] : 0.f, f, run.o[t][half]);
+          run.o[t][half + 2] = fmaf(some ? y[t * 16 + 8] : 0.f, f, run.o[t][half + 2]);
         }
       }
     }
