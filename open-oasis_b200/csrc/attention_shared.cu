@@ -990,29 +990,6 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   p->prefix_splits = 0;
   p->tensor = 0;
   p->reach = 0x7fffffff;
-  if (prefix) {
-    const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
-    const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
-    long long least = kTensorKeys;
-    if (p->tiles == 1 && (long long)a->groups * K > sms) least += (long long)a->groups * K - sms;
-    p->tensor = keys >= (least < kTensorKeysMost ? least : kTensorKeysMost) && pool_rows < (1LL << 31);
-    if (p->tensor) {
-      // one block for each SM, and at least 128 keys for each block
-      const long long pairs = ((long long)group_rows * p->per + 255) / 256;
-      p->tiles = (int)pairs;
-      p->reach = pairs * 256 < 0x7fffffff ? (int)pairs * 256 : 0x7fffffff;
-      const long long blocks = (long long)a->groups * K * pairs;
-      long long n = sms / blocks;
-      if (n > keys / 128) n = keys / 128;
-      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
-    } else {
-      // two blocks for each SM, and at least 128 keys for each block
-      const long long blocks = (long long)a->groups * K * p->tiles;
-      long long n = (2LL * sms + blocks - 1) / blocks;
-      if (n > keys / 128) n = keys / 128;
-      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
-    }
-  }
   // A row's own keys go to teams of four warps in ranges of one length, so that a row
   // longer than the others only has more of them: at least 256 keys, as many ranges as
   // make 12 teams for each SM where all rows have the hinted length. Where that length is
@@ -1033,6 +1010,36 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   if (each < 16) each = 16;
   p->own_units = (int)each;
   p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
+  if (prefix) {
+    const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
+    const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
+    long long least = kTensorKeys;
+    if (p->tiles == 1 && (long long)a->groups * K > sms) least += (long long)a->groups * K - sms;
+    p->tensor = keys >= (least < kTensorKeysMost ? least : kTensorKeysMost) && pool_rows < (1LL << 31);
+    if (p->tensor) {
+      // One block for each SM, and at least 128 keys for each block; two thirds of them where
+      // the own keys, in one range, can run beside them on the SMs that this leaves, since a
+      // block takes all of its SM's registers. All / two thirds, us: 64 rows behind 8192
+      // tokens, 16 heads of 64: 28.0 / 27.8 with up to 16 own tokens, 41.2 / 27.9 with 256;
+      // 32 / 8 heads of 128: 38.1 / 33.7, 49.8 / 34.2; 256 rows of 16 heads of 64: 53.8 / 56.1
+      // behind 8192 tokens, 43.2 / 41.3 behind 2048; with own keys in ranges, up to 2048 of
+      // them: 57.1 / 62.1.
+      const long long pairs = ((long long)group_rows * p->per + 255) / 256;
+      p->tiles = (int)pairs;
+      p->reach = pairs * 256 < 0x7fffffff ? (int)pairs * 256 : 0x7fffffff;
+      const long long blocks = (long long)a->groups * K * pairs;
+      long long n = sms / blocks;
+      if (p->own_splits == 1 && n >= 6) n = n * 2 / 3;
+      if (n > keys / 128) n = keys / 128;
+      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    } else {
+      // two blocks for each SM, and at least 128 keys for each block
+      const long long blocks = (long long)a->groups * K * p->tiles;
+      long long n = (2LL * sms + blocks - 1) / blocks;
+      if (n > keys / 128) n = keys / 128;
+      p->prefix_splits = (int)(n < 1 ? 1 : n > kMostSplits ? kMostSplits : n);
+    }
+  }
   // One pass where its blocks fill the GPU and a warp has at most 32 steps of own keys
   // for its eight queries and 16 of a prefix, one behind the other.
   const long long blocks = ((long long)a->rows * p->per + kWholeRows - 1) / kWholeRows * K;
