@@ -990,12 +990,18 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   p->prefix_splits = 0;
   p->tensor = 0;
   p->reach = 0x7fffffff;
+  const long long keys = prefix ? (long long)a->prefix_pages_hint * a->cache->page_size : 0;
+  if (prefix) {
+    const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
+    long long least = kTensorKeys;
+    if (p->tiles == 1 && (long long)a->groups * K > sms) least += (long long)a->groups * K - sms;
+    p->tensor = keys >= (least < kTensorKeysMost ? least : kTensorKeysMost) && pool_rows < (1LL << 31);
+  }
   // A row's own keys go to teams of four warps in ranges of one length, so that a row
-  // longer than the others only has more of them: at least 256 keys, as many ranges as
-  // make 12 teams for each SM where all rows have the hinted length. Where that length is
-  // small for the number of items (row, key head, eight heads), an item is one warp's: a
-  // block's lookups and its end then serve four items, and the longest row's warp takes
-  // four times as long. One warp / four, us, ragged rows in groups, so many items with rows
+  // longer than the others only has more of them. Where the hinted length is small for the
+  // number of items (row, key head, eight heads), an item is one warp's: a block's lookups
+  // and its end then serve four items, and the longest row's warp takes four times as long.
+  // One warp / four, us, ragged rows in groups, so many items with rows
   // of up to so many tokens behind their prefix: heads of 64: 272 items 12.6 / 13.6 (64), 20.5 /
   // 13.8 (256); 2512 items 19.5 / 28.8 (64), 30.4 / 32.6 (256), 80 / 47 (1024); 12544 items 47 /
   // 109 (64), 138 / 159 (1024). Heads of 128, where an SM holds half as many blocks: 536
@@ -1004,18 +1010,23 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const long long own = a->own_tokens_hint;
   const long long units = (own + kUnit - 1) / kUnit;
   p->team = units <= 8 + items * a->cache->head_dim / 8192 ? 1 : kOwnWarps;
-  long long n = p->team == 1 ? 1 : (12LL * sms + items - 1) / items;
+  // Ranges: as many as make 12 teams for each SM (heads of 128: 6) where all rows have the
+  // hinted length, up to twice as many where they would be longer than 1024 keys, each of
+  // at least 256. 12 / 24 teams, us: 64 rows alone, 16 heads of 64: 50.9 / 48.9 with up to
+  // 2000 tokens, 118 / 88 with 8000; behind 2048 shared ones 35.9 / 40.1 with 1000. 6 / 12,
+  // 32 / 8 heads of 128: 45.9 / 47.3, 98 / 78, 41.8 / 44.9. One range where a long prefix
+  // takes as long: 8 rows behind 2048 tokens, up to 1000 own ones, 25.7 -> 20.6 us.
+  const long long teams = 768 / a->cache->head_dim * sms;
+  long long n = units / 64 + (units % 64 != 0), most = (2 * teams + items - 1) / items;
+  if (n > most) n = most;
+  if (n * items < teams) n = (teams + items - 1) / items;
   if (n > kMostSplits) n = kMostSplits;
   long long each = (units + n - 1) / n;
   if (each < 16) each = 16;
+  if (p->team == 1 || (p->tensor && keys >= 2048 && units <= 64 && items <= 2LL * sms)) each = units > 16 ? units : 16;
   p->own_units = (int)each;
   p->own_splits = (int)(units > each ? (units + each - 1) / each : 1);
   if (prefix) {
-    const long long keys = (long long)a->prefix_pages_hint * a->cache->page_size;
-    const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
-    long long least = kTensorKeys;
-    if (p->tiles == 1 && (long long)a->groups * K > sms) least += (long long)a->groups * K - sms;
-    p->tensor = keys >= (least < kTensorKeysMost ? least : kTensorKeysMost) && pool_rows < (1LL << 31);
     if (p->tensor) {
       // One block for each SM, and at least 128 keys for each block; two thirds of them where
       // the own keys, in one range, can run beside them on the SMs that this leaves, since a
@@ -1045,7 +1056,7 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const long long blocks = ((long long)a->rows * p->per + kWholeRows - 1) / kWholeRows * K;
   const long long rows = (8 + p->per - 1) / p->per, steps = rows * ((own + kUnit - 1) / kUnit);
   p->whole = blocks >= 4LL * sms && steps <= 32 &&
-             (!prefix || (long long)a->prefix_pages_hint * a->cache->page_size <= 16 * kPrefixKeys);
+             keys <= 16 * kPrefixKeys;
 }
 
 size_t partial_bytes(const OasisSharedArgs* a, const SharedParams& p) {
