@@ -1011,13 +1011,13 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const long long units = (own + kUnit - 1) / kUnit;
   p->team = units <= 8 + items * a->cache->head_dim / 8192 ? 1 : kOwnWarps;
   // Ranges: as many as make 12 teams for each SM (heads of 128: 6) where all rows have the
-  // hinted length, up to twice as many where they would be longer than 1024 keys, each of
-  // at least 256. 12 / 24 teams, us: 64 rows alone, 16 heads of 64: 50.9 / 48.9 with up to
+  // hinted length, up to twice as many where they would be longer than 1024 keys (and the
+  // hint is not long for another group's prefix, 33.8 -> 41.2 us), each of at least 256. 12 / 24 teams, us: 64 rows alone, 16 heads of 64: 50.9 / 48.9 with up to
   // 2000 tokens, 118 / 88 with 8000; behind 2048 shared ones 35.9 / 40.1 with 1000. 6 / 12,
   // 32 / 8 heads of 128: 45.9 / 47.3, 98 / 78, 41.8 / 44.9. One range where a long prefix
   // takes as long: 8 rows behind 2048 tokens, up to 1000 own ones, 25.7 -> 20.6 us.
   const long long teams = 768 / a->cache->head_dim * sms;
-  long long n = units / 64 + (units % 64 != 0), most = (2 * teams + items - 1) / items;
+  long long n = own >= 2 * keys ? (units + 63) / 64 : 1, most = (2 * teams + items - 1) / items;
   if (n > most) n = most;
   if (n * items < teams) n = (teams + items - 1) / items;
   if (n > kMostSplits) n = kMostSplits;
