@@ -248,6 +248,40 @@ def test_long_prefixes(rows, heads, kv, dim, dtype, page):
     assert _lib.load().oasis_device_error(0) == 0
 
 
+RANGES = {  # (page, groups, key heads)
+    # own keys in one range that joins the ranges of a long prefix; a row that ends inside it
+    "one range": (64, lambda r: [(33, [2112 + n for n in (900, 5, 1, 440)] + [1000, 0])], 2),
+    # a warp for each item, beside a prefix on part of the SMs
+    "one warp": (16, lambda r: [(40, [640 + r.randint(0, 60) for _ in range(300)]), (0, [r.randint(0, 90) for _ in range(9)])], 8),
+    # rows of thousands of tokens, ragged, without a common prefix
+    "long rows": (128, lambda r: [(0, [5000, 17, 0, 2049, 1024, 1025, 300])], 2),
+    # many groups of few rows: their prefixes are too short for tensor memory
+    "many groups": (16, lambda r: [(25, [400 + r.randint(0, 30) for _ in range(r.randint(1, 2))]) for _ in range(100)], 2),
+    # ranges of own keys behind a prefix in ranges
+    "both": (32, lambda r: [(70, [2240 + 20 * n for n in range(60)]), (3, [1900, 96, 97])], 3),
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", RANGES)
+@pytest.mark.parametrize("per,dim,dtype", [(1, 64, BF16), (4, 128, FP16), (9, 64, FP16)])
+def test_ranges(name, per, dim, dtype):
+    """Each way that prefixes and own keys are split, with an infinity behind the rows' ends."""
+    page, groups, kv = RANGES[name]
+    c, seqs, plan, g = build(groups(random.Random(5)), page, kv, dim, dtype, layers=1)
+    q = queries(len(seqs), per * kv, dim, dtype, g)
+    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    check(got, q, c, 0, seqs)
+    assert torch.equal(got, paged.attention_shared(q, c, 0, ints(seqs), plan))
+    table, lengths = c.table.tolist(), c.lengths.tolist()
+    for s in seqs:  # a last page that no other row reads ends behind its row's last token
+        t = lengths[s]
+        if t % page and sum(table[s][t // page] in row for row in table) == 1:
+            c.pool[table[s][t // page], 0, :, :, t % page :] = math.inf
+    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    c.check()
+
+
 @pytest.mark.gpu
 def test_hints_only_choose_the_split():
     c, seqs, plan, g = build([(30, [500, 900, 700]), (0, [1200])], 16, 2, 64, BF16)
