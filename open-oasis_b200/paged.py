@@ -163,6 +163,10 @@ class PagedCache:
         self._c = bytes(c)  # the C struct, kept alive and passed as it is
         self._at = C.cast(self._c, C.c_void_p).value
 
+    def __reduce__(self):
+        """Copied and stored as its tensors: the struct holds their addresses."""
+        return PagedCache.from_tensors, (self.pool, self.table, self.lengths, self.refs)
+
     def reserve(self, seqs: torch.Tensor, cu: torch.Tensor, stream=None) -> torch.Tensor:
         """Room for cu[i + 1] - cu[i] more tokens behind sequence seqs[i]; returns
         each one's length before (-1: refused, see `status`), for `write`."""

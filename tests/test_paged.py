@@ -2,7 +2,9 @@
 and over random runs of calls; refusals; bad indexes; graph replay."""
 from __future__ import annotations
 
+import copy
 import ctypes as C
+import io
 import os
 import random
 import subprocess
@@ -338,6 +340,25 @@ def test_graph_replay_and_side_stream():
     torch.cuda.current_stream().wait_stream(side)
     o.free([2, 3, 4])
     same(c, o)
+
+
+@pytest.mark.gpu
+def test_copies_and_stored_caches_are_their_own():
+    """A deep copy, or a cache stored and loaded, changes its own tensors and not the first's."""
+    c = paged.PagedCache(8, 16, 1, 1, 64, 3, 4, device=DEV)
+    seqs, cu = ints([0]), ints([0, 20])
+    c.reserve(seqs, cu)
+    buffer = io.BytesIO()
+    torch.save(c, buffer)
+    buffer.seek(0)
+    for other in (copy.deepcopy(c), torch.load(buffer, weights_only=False)):
+        assert torch.equal(other.table, c.table) and other.table.data_ptr() != c.table.data_ptr()
+        other.reserve(seqs, cu)
+        assert other.lengths.tolist() == [40, 0, 0] and c.lengths.tolist() == [20, 0, 0]
+        assert int(other.refs.sum()) == 3 and int(c.refs.sum()) == 2
+    same = copy.copy(c)
+    same.reserve(seqs, cu)
+    assert c.lengths.tolist() == [40, 0, 0]
 
 
 @pytest.mark.gpu
