@@ -783,11 +783,10 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 6 : 3) shared_whole_kernel
     const int group = group_of[x];
     const int tokens = begin_of[x];
     if (row_of[x] < 0) break;
-    // the rows of the group are consecutive
-    int after = x;
-#pragma unroll
-    for (int i = 0; i < kWholeRows; i += 32)
-      after += __popc(__ballot_sync(0xffffffffu, i + lane >= x && group_of[i + lane] == group && row_of[i + lane] >= 0));
+    // up to the first row of another group (rows of none lie before the groups and behind them)
+    static_assert(kWholeRows == 32, "a lane for each query");
+    const unsigned others = __ballot_sync(0xffffffffu, lane > x && (group_of[lane] != group || row_of[lane] < 0));
+    const int after = others ? __ffs(others) - 1 : kWholeRows;
     if (tokens == 0) {
       x = after;
       continue;

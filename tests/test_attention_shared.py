@@ -137,6 +137,31 @@ def test_plan_is_checked():
 
 # --------------------------------------------------------------------- on a GPU --
 
+# How a call is carried out goes by its sizes: small batches read each row by itself, larger
+# ones run one of three kernels for the prefix. These make a small batch take each way.
+WAYS = ["as it is", "tensor memory", "mma", "one pass"]
+
+
+def run(way, q, c, layer, seqs, plan):
+    """The call with hints, and with rows of an empty sequence behind the plan's, that
+    lead it the given way; the results of the rows in `seqs`."""
+    hints, extra = (plan.longest, plan.most_pages), 0
+    heads = q.shape[1]
+    if way == "tensor memory":
+        plan.most_pages = 1 << 16
+    elif way != "as it is":
+        read = max(1, plan.most_pages) * c.page_size * c.kv_heads * c.head_dim * 4
+        extra = 120_000_000 // read + plan.groups + (20_000 // heads if way == "one pass" else 0)
+        plan.longest = 1 if way == "one pass" else 1 << 20
+    lengths = c.lengths.tolist()
+    empty = next(s for s in range(c.sequences) if lengths[s] == 0)
+    more = torch.zeros(extra, heads, c.head_dim, dtype=q.dtype, device=DEV)
+    got = paged.attention_shared(torch.cat([q, more]), c, layer, ints(list(seqs) + [empty] * extra), plan)
+    plan.longest, plan.most_pages = hints
+    assert not bool(got[len(seqs) :].any())
+    return got[: len(seqs)]
+
+
 GROUPS = {
     "long prefix": [(33, [600, 540, 528]), (80, [1290, 1281])],
     "long and short": [(40, [645, 100, 0, 700, 639, 641]), (2, [33])],
@@ -162,8 +187,8 @@ def test_groups(name, heads, kv, dim, dtype, page):
               for p, ls in GROUPS[name]]
     c, seqs, plan, g = build(groups, page, kv, dim, dtype)
     q = queries(len(seqs), heads, dim, dtype, g)
-    got = paged.attention_shared(q, c, 1, ints(seqs), plan)
-    check(got, q, c, 1, seqs)
+    for way in WAYS:
+        check(run(way, q, c, 1, seqs, plan), q, c, 1, seqs)
     alone = paged.SharedPlan([], [], plan.longest, DEV)
     check(paged.attention_shared(q, c, 1, ints(seqs), alone), q, c, 1, seqs)
     c.check()
@@ -208,6 +233,7 @@ def test_many_rows_with_few_keys(shape, heads, kv, dim, dtype, page):
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,heads,kv,dim,dtype,page", [
     (300, 2, 2, 64, BF16, 16), (70, 12, 3, 128, BF16, 64), (40, 7, 1, 64, FP16, 48), (140, 2, 1, 128, FP16, 128), (3, 4, 4, 64, BF16, 256),
+    (40, 28, 4, 64, FP16, 48), (60, 4, 4, 64, BF16, 256),
 ])
 def test_long_prefixes(rows, heads, kv, dim, dtype, page):
     """The tensor-memory kernel: both tiles, several ranges, pages above and below a block,
@@ -250,13 +276,13 @@ def test_long_prefixes(rows, heads, kv, dim, dtype, page):
 
 RANGES = {  # (page, groups, key heads)
     # own keys in one range that joins the ranges of a long prefix; a row that ends inside it
-    "one range": (64, lambda r: [(33, [2112 + n for n in (900, 5, 1, 440)] + [1000, 0])], 2),
+    "one range": (64, lambda r: [(33, [2112 + n for n in (900, 5, 1, 440)] + [1000, 0])], 16),
     # a warp for each item, beside a prefix on part of the SMs
     "one warp": (16, lambda r: [(40, [640 + r.randint(0, 60) for _ in range(300)]), (0, [r.randint(0, 90) for _ in range(9)])], 8),
     # rows of thousands of tokens, ragged, without a common prefix
     "long rows": (128, lambda r: [(0, [5000, 17, 0, 2049, 1024, 1025, 300])], 2),
     # many groups of few rows: their prefixes are too short for tensor memory
-    "many groups": (16, lambda r: [(25, [400 + r.randint(0, 30) for _ in range(r.randint(1, 2))]) for _ in range(100)], 2),
+    "many groups": (16, lambda r: [(25, [400 + r.randint(0, 30) for _ in range(r.randint(1, 4))]) for _ in range(100)], 8),
     # ranges of own keys behind a prefix in ranges
     "both": (32, lambda r: [(70, [2240 + 20 * n for n in range(60)]), (3, [1900, 96, 97])], 3),
 }
@@ -278,7 +304,13 @@ def test_ranges(name, per, dim, dtype):
         t = lengths[s]
         if t % page and sum(table[s][t // page] in row for row in table) == 1:
             c.pool[table[s][t // page], 0, :, :, t % page :] = math.inf
-    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    graph, at = torch.cuda.CUDAGraph(), ints(seqs)
+    with torch.cuda.graph(graph):
+        again = paged.attention_shared(q, c, 0, at, plan)
+    for _ in range(3):
+        again.zero_()
+        graph.replay()
+    check(again, q, c, 0, seqs)
     c.check()
 
 
@@ -292,19 +324,21 @@ def test_hints_only_choose_the_split():
 
 
 @pytest.mark.gpu
-def test_rows_outside_the_groups_and_named_twice():
+@pytest.mark.parametrize("way", WAYS)
+def test_rows_outside_the_groups_and_named_twice(way):
     c, seqs, _, g = build([(2, [40, 50, 33])], 16, 1, 64, BF16)
     plan = paged.SharedPlan([2], [2], 64, DEV)
     plan.group_start += 1  # rows 1 and 2
     order = [seqs[2], seqs[0], seqs[1], seqs[0], seqs[2]]
     q = queries(5, 2, 64, BF16, g)
-    check(paged.attention_shared(q, c, 0, ints(order), plan), q, c, 0, order)
+    check(run(way, q, c, 0, order, plan), q, c, 0, order)
 
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
-def test_what_lies_behind_a_sequence_takes_no_part(dim, bad):
+@pytest.mark.parametrize("way", WAYS)
+def test_what_lies_behind_a_sequence_takes_no_part(way, dim, bad):
     """NaN in pages behind a sequence's last token, and in the prefix behind a shorter
     row; NaN and empty results where the formula has them."""
     groups = [(3, [20, 70, 52, 0, 48]), (0, [7])]
@@ -317,20 +351,21 @@ def test_what_lies_behind_a_sequence_takes_no_part(dim, bad):
     unused = [p for p in range(c.pages) if all(p not in r for r in lists)]
     c.pool[unused] = bad
     q = queries(6, 6, dim, BF16, g)
-    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    got = run(way, q, c, 0, seqs, plan)
     check(got, q, c, 0, seqs)
     c.pool[lists[seqs[1]][2], :, :, :, 5] = bad  # token 37 of the prefix: rows 1, 2 and 4 see it, row 0 does not
-    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    got = run(way, q, c, 0, seqs, plan)
     want = check(got, q, c, 0, seqs, rows=[0, 3, 5])
     assert torch.equal(torch.isnan(got), torch.isnan(want)) and bool(torch.isnan(want[[1, 2, 4]]).any())
     q[1] = math.nan
-    got = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    got = run(way, q, c, 0, seqs, plan)
     check(got, q, c, 0, seqs, rows=[0, 3, 5])
     assert bool(torch.isnan(got[1]).all())
 
 
 @pytest.mark.gpu
-def test_lowest_scores():
+@pytest.mark.parametrize("way", WAYS)
+def test_lowest_scores(way):
     """Keys that score -inf or the lowest value: in the whole prefix, in a row's own part."""
     c, seqs, plan, g = build([(4, [70, 100])], 16, 1, 64, BF16)
     q = queries(2, 2, 64, BF16, g)
@@ -338,22 +373,23 @@ def test_lowest_scores():
     c.pool[..., 0] = torch.where(torch.arange(2, device=DEV)[None, None, :, None, None] == 0, 0, c.pool[..., 0])
     common = c.table[seqs[0], :4].long()
     c.pool[common, :, 0, :, :, 0] = -math.inf
-    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    check(run(way, q, c, 0, seqs, plan), q, c, 0, seqs)
     c.pool[common, :, 0, :, :, 0] = torch.finfo(BF16).min
-    check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
+    check(run(way, q, c, 0, seqs, plan), q, c, 0, seqs)
     c.pool[:, :, 0, :, :, 0] = -math.inf
-    assert bool(torch.isnan(paged.attention_shared(q, c, 0, ints(seqs), plan)).all())  # as the formula: 0 / 0
+    assert bool(torch.isnan(run(way, q, c, 0, seqs, plan)).all())  # as the formula: 0 / 0
 
 
 @pytest.mark.gpu
-def test_bad_indexes_are_left_out():
+@pytest.mark.parametrize("way", WAYS)
+def test_bad_indexes_are_left_out(way):
     c, seqs, plan, g = build([(2, [40, 40]), (0, [64, 20])], 16, 1, 64, BF16)
     q = queries(4, 1, 64, BF16, g)
-    good = paged.attention_shared(q, c, 0, ints(seqs), plan)
+    good = run(way, q, c, 0, seqs, plan)
     table = c.table.clone()
     c.table[seqs[2], 1] = 1 << 30
     c.table[seqs[3], :2] = ints([-1, c.pages])
-    got = paged.attention_shared(q, c, 0, ints([seqs[0], 99, seqs[2], seqs[3]]), plan)
+    got = run(way, q, c, 0, [seqs[0], 99, seqs[2], seqs[3]], plan)
     torch.cuda.synchronize()
     assert torch.equal(got[0], good[0]) and not bool(got[1].any()) and not bool(got[3].any())
     assert int(c.status.item()) == paged.BAD_SEQUENCE | paged.BAD_PAGE
