@@ -983,13 +983,27 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const int K = a->cache->kv_heads;
   p->per = a->heads / K;
   p->head_tiles = (p->per + 7) / 8;
-  const bool prefix = a->groups > 0 && a->prefix_pages_hint > 0;
+  bool prefix = a->groups > 0 && a->prefix_pages_hint > 0;
+  long long own = a->own_tokens_hint;
+  long long keys = prefix ? (long long)a->prefix_pages_hint * a->cache->page_size : 0;
+  // Where sharing would save little reading (and what is read again comes from L2), each
+  // row reads its prefix with its own keys: one kernel, and nothing waits for another. Shared
+  // / alone, us, up to 40 own tokens, 16 heads of 64: 3 rows behind 144 tokens 12.0 / 5.6, 8
+  // behind 500 (14 MB saved) 11.2 / 11.7, 16 behind 500 (31 MB) 11.4 / 14.7; 32 / 8 heads of
+  // 128: 16 behind 500 14.5 / 12.7, 32 behind 500 (63 MB) 15.5 / 19.0. Groups cost the prefix
+  // kernel more: 16 of up to 4 rows, 500 tokens, 29.8 / 15.7.
+  const double saved = ((double)a->rows - a->groups) * keys * K * a->cache->head_dim * 4;  // bytes
+  if (prefix && saved <= ((a->cache->head_dim == 64 ? 24 : 48) + 2 * (a->groups < 16 ? a->groups : 16)) * 1048576.0) {
+    own += keys;
+    keys = 0;
+    prefix = false;
+  }
+  p->groups = prefix ? a->groups : 0;
   const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
   p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);
   p->prefix_splits = 0;
   p->tensor = 0;
   p->reach = 0x7fffffff;
-  const long long keys = prefix ? (long long)a->prefix_pages_hint * a->cache->page_size : 0;
   if (prefix) {
     const long long pool_rows = (long long)a->cache->pages * a->cache->layers * 2 * K * a->cache->page_size;
     long long least = kTensorKeys;
@@ -1006,7 +1020,6 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   // 109 (64), 138 / 159 (1024). Heads of 128, where an SM holds half as many blocks: 536
   // items 18.9 / 23.1 (64), 24.1 / 25.2 (256), 83 / 54 (4096); 6272 items 56 / 117 (64), 138 / 165 (1024).
   const long long items = (long long)a->rows * K * p->head_tiles;
-  const long long own = a->own_tokens_hint;
   const long long units = (own + kUnit - 1) / kUnit;
   p->team = units <= 8 + items * a->cache->head_dim / 8192 ? 1 : kOwnWarps;
   // Ranges: as many as make 12 teams for each SM (heads of 128: 6) where all rows have the
@@ -1154,7 +1167,6 @@ int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream) {
                   "attention_shared: stride %lld is not a positive multiple of 8 elements", s);
   SharedParams p;
   plan(a, &p);
-  p.groups = a->groups > 0 && a->prefix_pages_hint > 0 ? a->groups : 0;
   const long long blocks = (long long)a->groups * c->kv_heads * (p.prefix_splits ? p.prefix_splits : 1) * p.tiles;
   const long long items = (long long)a->rows * c->kv_heads * p.head_tiles * p.own_splits;
   OASIS_REQUIRE(blocks < (1LL << 31) && items < (1LL << 31), "attention_shared: %d rows of %d heads are too many",
