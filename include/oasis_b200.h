@@ -631,7 +631,8 @@ int oasis_attention_prompt(const OasisPromptArgs* a, oasis_stream_t stream);
  * and set BAD_PAGE.
  * Group g is the rows [group_start[g], group_start[g + 1]) (device, non-decreasing);
  * the first prefix_pages[g] (device) entries of its sequences' table rows have to be
- * the same pages (as oasis_pages_fork leaves them): they are read once for the group.
+ * the same pages (as oasis_pages_fork leaves them): they are read once for the group,
+ * unless the batch is so small that this would save nothing.
  * Rows outside all groups share nothing; groups = 0 is attention without sharing. The
  * hints (largest group, longest prefix, most tokens behind a prefix) choose tiles and
  * splits and nothing else; prefix_pages_hint = 0 shares nothing. The call's workspace

@@ -16,10 +16,11 @@
 // two steps of keys in flight per warp and the rows' different lengths are the rest. It
 // runs beside the prefix kernel. With one range it joins the prefix's and
 // writes the result; otherwise shared_join_kernel does, a warp per (row, head).
-// 64 rows behind 8192 shared tokens, up to 1024 own ones, 32 / 8 heads of 128: 51 us, about
-// 25 for the prefix, 23 for the own keys beside and behind it and 10 for the join; the
-// bytes alone would take 10.
+// 64 rows behind 8192 shared tokens, up to 1024 own ones, 32 / 8 heads of 128: 49 us, about
+// 25 for the prefix, the own keys beside and behind it and 8 to 10 for the join; the bytes
+// alone would take 10.
 // shared_whole_kernel: both in one pass where rows are many and short.
+// Small batches run the own kernel alone, their prefixes read with the rows' own keys.
 #include "../../include/oasis_b200.h"
 #include "attention_rows.cuh"
 #include "attention_shared.cuh"

@@ -12,8 +12,8 @@
 //
 // Bound: for a group of at least 256 queries the softmax's pipes, as there; for small
 // ones the latency of a range's blocks, S, softmax and P V one behind the other. 64 rows
-// of 32 / 8 heads of 128 behind 8192 tokens: about 25 us for the 18 ranges of each key
-// head, of which 6 are the block's start (the longest row, Q, the first pages).
+// of 32 / 8 heads of 128 behind 8192 tokens: about 25 us with 18 ranges for each key head,
+// of which 6 are the block's start (the longest row, Q, the first pages).
 #include "../../include/oasis_b200.h"
 #include "attention_shared.cuh"
 #include "attention_tc.cuh"
