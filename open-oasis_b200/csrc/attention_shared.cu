@@ -999,6 +999,8 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
     keys = 0;
     prefix = false;
   }
+  const long long room = (long long)a->cache->width * a->cache->page_size;  // of a sequence, below 2^31
+  if (own > room) own = room;
   p->groups = prefix ? a->groups : 0;
   const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
   p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);

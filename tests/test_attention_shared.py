@@ -105,6 +105,8 @@ def test_arguments_are_checked(cache, kw, text):
 def test_workspace_is_asked_for():
     lib = _lib.load()
     a, _ = _args(rows=2, groups=1, group_start=16, prefix_pages=16, group_rows_hint=2, prefix_pages_hint=40)
+    assert lib.oasis_attention_shared_workspace_size(C.byref(a)) == 0  # each row by itself, in one range
+    a, _ = _args(rows=2, groups=1, group_start=16, prefix_pages=16, group_rows_hint=2, prefix_pages_hint=20000)
     size = lib.oasis_attention_shared_workspace_size(C.byref(a))
     assert size > 0
     for ws, n in ((0, size), (16, size - 1)):
@@ -114,6 +116,15 @@ def test_workspace_is_asked_for():
     assert lib.oasis_attention_shared_workspace_size(C.byref(a)) == 0
     assert lib.oasis_attention_shared(C.byref(a), None) == 0
     assert lib.oasis_attention_shared(None, None) == -1
+
+
+def test_workspace_of_the_largest_hints():
+    """As many groups as rows save nothing: hints of any size ask for ranges of rows that exist."""
+    lib, most = _lib.load(), (1 << 31) - 1
+    for groups in (1, 2):
+        a, _ = _args(rows=2, groups=groups, group_start=16, prefix_pages=16, group_rows_hint=most,
+                     prefix_pages_hint=most, own_tokens_hint=most)
+        assert 0 <= lib.oasis_attention_shared_workspace_size(C.byref(a)) <= 2 * 128 * (64 * 4 + 8)
 
 
 def test_struct_layout_matches_c():
@@ -318,7 +329,8 @@ def test_ranges(name, per, dim, dtype):
 def test_hints_only_choose_the_split():
     c, seqs, plan, g = build([(30, [500, 900, 700]), (0, [1200])], 16, 2, 64, BF16)
     q = queries(4, 4, 64, BF16, g)
-    for longest, rows, pages in ((1, 1, 1), (1 << 20, 1000, 1), (900, 1, 4000), (10, 3, 0)):
+    most = (1 << 31) - 1
+    for longest, rows, pages in ((1, 1, 1), (1 << 20, 1000, 1), (900, 1, 4000), (10, 3, 0), (most, 1, 1)):
         plan.longest, plan.most_rows, plan.most_pages, plan.least_pages = longest, rows, pages, 0
         check(paged.attention_shared(q, c, 0, ints(seqs), plan), q, c, 0, seqs)
 
