@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       if (mine) p.part_ml[slot_of(lane)] = make_float2(-INFINITY, 0.f);
     } else if (ok && wait_for(&pv_done[t], (blocks - 1) & 1, kDevTimeoutAccFull)) {
       tc_fence_after();
-      if (m == -INFINITY && finite_f(l)) l = 0.f;  // no key that counts: masked ones left 2^-125 each
+      if (m == -INFINITY && finite_f(l)) l = 0.f;  // no key that counts: masked ones left 2^-136 each in the sum
       if (mine) p.part_ml[slot_of(lane)] = make_float2(m, l);
       // O through this tile's Q, which no product reads any more: 32 columns of 32 rows,
       // so that a store covers four rows' 128 bytes

@@ -367,3 +367,26 @@ def test_python_checks():
     with pytest.raises(_lib.OasisError, match="kv_heads=2"):
         call(q[:, :3], k, v, cu, 10)
     assert call(q[:0], k[:0], v[:0], ints([0]), 0).shape == (0, 4, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(2, 1, 64, BF16), (2, 1, 128, BF16), (3, 1, 64, BF16), (2, 1, 64, FP16)])
+def test_large_values_that_are_not_seen_change_no_bit(hint, heads, kv, dim, dtype):
+    """Finite keys and values up to the type's largest in later rows of a sequence, in its
+    neighbours and behind the last sequence: the rows that do not see them keep every bit
+    that they have with zeros there."""
+    lengths = [200, 130, 61]
+    q, k, v = inputs(lengths, heads, kv, dim, dtype, seed=17, extra=130)
+    hidden = torch.zeros(q.shape[0], dtype=torch.bool, device=DEV)
+    for a, b in ((150, 200), (300, 330), (391, 521)):
+        hidden[a:b] = True
+    cu = ints(starts(lengths))
+    k[hidden], v[hidden] = 0, 0
+    want = paged.attention_prompt(q, k, v, cu, hint)
+    assert bool(torch.isfinite(want[:391]).all())
+    for size in (1e30, 1e36, 3.3e38) if dtype == BF16 else (6e4,):
+        k[hidden], v[hidden] = size, size
+        v[hidden] *= torch.where(torch.arange(dim, device=DEV) % 2 == 0, 1, -1).to(dtype)
+        got = paged.attention_prompt(q, k, v, cu, hint)
+        assert torch.equal(got[~hidden], want[~hidden]), size

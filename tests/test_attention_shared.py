@@ -554,3 +554,30 @@ def test_python_checks():
     with pytest.raises(_lib.OasisError, match="layer=2"):
         call(q, c, 2, at, plan)
     assert call(q[:0], c, 0, at[:0], paged.SharedPlan([], [], 1, DEV)).shape == (0, 1, 64)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, BF16), (64, FP16)])
+@pytest.mark.parametrize("way", WAYS)
+def test_large_values_that_are_not_seen_change_no_bit(way, dim, dtype):
+    """Finite keys and values up to the type's largest behind a sequence's last token and in
+    the prefix behind a shorter row: the rows that do not see them keep every bit that they
+    have with zeros there."""
+    groups = [(15, [250, 100, 0, 17, 241, 242]), (15, [230, 225]), (0, [7])]
+    c, seqs, plan, g = build(groups, 16, 2, dim, dtype)
+    lists, lengths = c.table.tolist(), c.lengths.tolist()
+    places = [(lists[seqs[0]][t // 16], t % 16) for t in range(100, 240)]  # rows 0, 4 and 5 see these
+    for b in (0, 4, 5, 6, 8):
+        t = lengths[seqs[b]]
+        places += [(lists[seqs[b]][t // 16], x) for x in range(t % 16, 16)]
+    pages, slots = (torch.tensor(x, device=DEV) for x in zip(*places))
+    q = queries(len(seqs), 6, dim, dtype, g)
+    blind = [1, 2, 3, 6, 7, 8]
+    fill = lambda x: c.pool.__setitem__((pages, slice(None), slice(None), slice(None), slots), x)  # noqa: E731
+    fill(0)
+    want = run(way, q, c, 0, seqs, plan)
+    check(want, q, c, 0, seqs)
+    for size in (1e30, 1e36, 3.3e38) if dtype == BF16 else (6e4,):
+        fill(size)
+        assert torch.equal(run(way, q, c, 0, seqs, plan)[blind], want[blind]), size
+    c.check()
