@@ -413,7 +413,9 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       if (mine) p.part_ml[slot_of(lane)] = make_float2(-INFINITY, 0.f);
     } else if (ok && wait_for(&pv_done[t], (blocks - 1) & 1, kDevTimeoutAccFull)) {
       tc_fence_after();
-      if (m == -INFINITY && finite_f(l)) l = 0.f;  // no key that counts: masked ones left 2^-136 each in the sum
+      // No score above -inf: the masked keys left at most 2^-136 each in the sum. Only a score of
+      // NaN, which the maximum passes over, leaves more (or NaN), and then the row is NaN.
+      if (m == -INFINITY) l = l < 1.f ? 0.f : __int_as_float(0x7fffffff);
       if (mine) p.part_ml[slot_of(lane)] = make_float2(m, l);
       // O through this tile's Q, which no product reads any more: 32 columns of 32 rows,
       // so that a store covers four rows' 128 bytes

@@ -581,3 +581,19 @@ def test_large_values_that_are_not_seen_change_no_bit(way, dim, dtype):
         fill(size)
         assert torch.equal(run(way, q, c, 0, seqs, plan)[blind], want[blind]), size
     c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("at", [128, 129, 256, 260])
+def test_a_score_of_nan_alone_in_a_range(way, dim, at):
+    """A shorter row's last token in the prefix is a NaN key at or near the start of a range,
+    so that its range may hold no other key that it sees: its result is NaN all the same."""
+    c, seqs, plan, g = build([(20, [at + 1, 400, at])], 16, 2, dim, BF16)
+    page = c.table[seqs[1]].tolist()[at // 16]
+    c.pool[page, 0, 0, :, at % 16, 5] = math.nan
+    q = queries(3, 4, dim, BF16, g)
+    got = run(way, q, c, 0, seqs, plan)
+    assert bool(torch.isnan(got[:2]).all())
+    check(got, q, c, 0, seqs, rows=[2])
