@@ -38,7 +38,7 @@
 #include "attention_prompt.cuh"
 #include "attention_tc.cuh"
 #include "gemm.cuh"
-#include "pages.cuh"
+#include "prompt_unit.cuh"
 #include "status.h"
 
 namespace oasis {
@@ -65,50 +65,7 @@ struct Cfg {
   static constexpr int O_COL = kApart ? 384 : 256;    // + D per tile
 };
 
-// What the block's two tiles cover. Every role works it out alike from cu.
-struct Unit {
-  int head[2], r0[2];       // tile t: its head and first row
-  int begin;                // first key of block 0
-  int first[2], last[2];    // tile t takes key blocks [first, last)
-  int blocks;
-};
-
-__device__ __forceinline__ Unit make_unit(const PromptParams& p, int pair_heads, int end, int x, int rt) {
-  Unit u;
-  const int rows = pair_heads ? kTile : 2 * kTile;
-  int low[2];
-  u.begin = 0x7fffffff;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    u.head[t] = pair_heads ? 2 * x + t : x;
-    u.r0[t] = rt * rows + (pair_heads ? 0 : t * kTile);
-    // the first row of the tile that belongs to a sequence, and that sequence's start
-    int lo = 0x7fffffff;
-    if (t == 1 && pair_heads) {
-      lo = low[0];
-    } else if (u.r0[t] < end) {
-      const int a = p.cu[last_not_above(p.cu, p.n, u.r0[t])];
-      if (a > u.r0[t]) {
-        if (a < u.r0[t] + kTile && a < end) lo = a;
-      } else if (a >= 0) {
-        lo = a;
-      }
-    }
-    low[t] = lo;
-    u.begin = min(u.begin, lo);
-  }
-  u.blocks = 0;
-#pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    u.first[t] = u.last[t] = 0;
-    if (low[t] != 0x7fffffff) {
-      u.first[t] = (low[t] - u.begin) / kTile;
-      u.last[t] = (min(u.r0[t] + kTile, end) - u.begin + kTile - 1) / kTile;
-      u.blocks = max(u.blocks, u.last[t]);
-    }
-  }
-  return u;
-}
+static_assert(kPromptTile == kTile, "tiles");
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
@@ -124,7 +81,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
   const int head_units = pair_heads ? p.heads / 2 : p.heads;
   const int tile_rows = pair_heads ? kTile : 2 * kTile;
   const int at = blockIdx.x / head_units;
-  const Unit u = make_unit(p, pair_heads, end, blockIdx.x - at * head_units, (p.rows + tile_rows - 1) / tile_rows - 1 - at);
+  const PromptUnit u = prompt_unit(p.cu, p.n, pair_heads, end, blockIdx.x - at * head_units,
+                                   (p.rows + tile_rows - 1) / tile_rows - 1 - at);
   if (u.blocks == 0) return;  // the whole block
 
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -190,13 +148,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         ++issued;
         return true;
       };
-      load(sQ, &tmQ, &q_full[0], u.head[0], u.r0[0]);
+      if (u.has(0)) load(sQ, &tmQ, &q_full[0], u.head[0], u.r0[0]);
       ok = next();
-      load(sQ + C::TILE_BYTES, &tmQ, &q_full[1], u.head[1], u.r0[1]);
+      if (u.has(1)) load(sQ + C::TILE_BYTES, &tmQ, &q_full[1], u.head[1], u.r0[1]);
       while (ok && issued < total) ok = next();
       if (!ok) {  // gave up: the copies in flight land before the block ends
-        wait_for(&q_full[0], 0, kDevTimeoutTmaFull);
-        wait_for(&q_full[1], 0, kDevTimeoutTmaFull);
+        for (int t = 0; t < 2; ++t)
+          if (u.has(t)) wait_for(&q_full[t], 0, kDevTimeoutTmaFull);
         for (int i = max(0, issued - C::STAGES); i < issued; ++i)
           wait_for(&kv_full[i % C::STAGES], (i / C::STAGES) & 1, kDevTimeoutTmaFull);
       }

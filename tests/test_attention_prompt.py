@@ -390,3 +390,72 @@ def test_large_values_that_are_not_seen_change_no_bit(hint, heads, kv, dim, dtyp
         v[hidden] *= torch.where(torch.arange(dim, device=DEV) % 2 == 0, 1, -1).to(dtype)
         got = paged.attention_prompt(q, k, v, cu, hint)
         assert torch.equal(got[~hidden], want[~hidden]), size
+
+
+def test_what_a_block_covers():
+    """The tiles of a block, over many offsets: each row's keys lie in its tile's key blocks,
+    and a tile's queries are fetched exactly where a product waits for them, so that no copy
+    is left on its way when a block without a second (or a first) tile ends."""
+    src = f'#include <stdio.h>\n#include <stdlib.h>\n#include "{ROOT}/open-oasis_b200/csrc/prompt_unit.cuh"\n' + r'''
+    using namespace oasis;
+    int main() {
+      srand(1);
+      int one_tile[2] = {0, 0};
+      for (int run = 0; run < 4000; ++run) {
+        int cu[9], n = 1 + rand() % 8;
+        cu[0] = run % 3 ? 0 : rand() % 400;
+        for (int i = 0; i < n; ++i) cu[i + 1] = cu[i] + (rand() % 4 ? rand() % (run % 2 ? 40 : 300) : 0);
+        const int rows = 1 + rand() % (cu[n] + 300), end = rows < cu[n] ? rows : cu[n];
+        for (int pair = 0; pair < 2; ++pair) {
+          const int tile_rows = pair ? kPromptTile : 2 * kPromptTile;
+          for (int rt = 0; rt < (rows + tile_rows - 1) / tile_rows; ++rt) {
+            const PromptUnit u = prompt_unit(cu, n, pair, end, 0, rt);
+            int blocks = 0;
+            for (int t = 0; t < 2; ++t) {
+              bool waited = false;  // as the warp that issues the products walks the blocks
+              for (int j = 0; j < u.blocks; ++j)
+                if (j >= u.first[t] && j < u.last[t]) waited = true;
+              if (waited != u.has(t)) printf("waits %d %d\n", run, t);
+              if (u.last[t] > blocks) blocks = u.last[t];
+              if (u.blocks > 0 && !u.has(t)) ++one_tile[t];
+              for (int r = u.r0[t]; r < u.r0[t] + kPromptTile && r < end; ++r) {
+                if (r < cu[0]) continue;
+                const int a = cu[last_not_above(cu, n, r)];
+                if (a < u.begin + u.first[t] * kPromptTile || r >= u.begin + u.last[t] * kPromptTile)
+                  printf("keys %d %d\n", run, r);
+              }
+            }
+            if (blocks != u.blocks || u.blocks < 0) printf("blocks %d\n", run);
+          }
+        }
+      }
+      printf(one_tile[0] > 0 && one_tile[1] > 0 ? "done\n" : "no block of one tile\n");
+      return 0;
+    }'''
+    with tempfile.TemporaryDirectory() as d:
+        f, exe = os.path.join(d, "u.cpp"), os.path.join(d, "u")
+        open(f, "w").write(src)
+        subprocess.run(["g++", "-std=c++17", "-fsanitize=undefined", "-fno-sanitize-recover", f, "-o", exe], check=True)
+        assert subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split("\n")[:-1] == ["done"]
+
+
+def test_queries_are_fetched_only_for_tiles_that_wait():
+    """In the kernel: each copy into a tile's Q stands behind that tile's `has`."""
+    text = open(f"{ROOT}/open-oasis_b200/csrc/attention_prompt_tc.cu").read()
+    loads = [line for line in text.splitlines() if "&tmQ, &q_full" in line]
+    assert len(loads) == 2 and all(f"if (u.has({t})) load(" in line for t, line in enumerate(loads))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("begin,lengths,extra", [(0, [300], 0), (0, [513], 200), (140, [300], 0), (400, [20, 250], 90)])
+def test_blocks_of_one_tile(dim, begin, lengths, extra):
+    """Heads that do not pair: blocks whose second tile, or whose first, has no row."""
+    cu = starts(lengths, begin)
+    q, k, v = inputs([cu[-1]], 3, 1, dim, BF16, seed=20, extra=extra)
+    out = torch.full(q.shape, 7.0, dtype=BF16, device=DEV)
+    for _ in range(3):
+        paged.attention_prompt(q, k, v, ints(cu), 1 << 20, out=out)
+    check(out, q, k, v, cu)
+    assert bool((out[:begin] == 7).all()) and bool((out[cu[-1] :] == 7).all())
+    assert _lib.load().oasis_device_error(0) == 0
