@@ -1002,8 +1002,16 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
   const long long room = (long long)a->cache->width * a->cache->page_size;  // of a sequence, below 2^31
   if (own > room) own = room;
   p->groups = prefix ? a->groups : 0;
-  const int group_rows = a->group_rows_hint < 1 ? 1 : a->group_rows_hint;
-  p->tiles = (int)(((long long)group_rows * p->per + kPrefixRows - 1) / kPrefixRows);
+  // A group has no more rows than the batch, whatever the hint; and what tiles do not cover is
+  // covered all the same (they go on behind their last one, or leave rows to the own keys),
+  // so that a launch has at most 2^30 of them.
+  const long long hint = a->group_rows_hint < 1 ? 1 : a->group_rows_hint, group_rows = hint < a->rows ? hint : a->rows;
+  const long long most_tiles = prefix ? (1LL << 30) / ((long long)a->groups * K) : 1;
+  auto tiles = [&](int queries) {
+    const long long n = (group_rows * p->per + queries - 1) / queries;
+    return (int)(n < most_tiles ? n : most_tiles > 1 ? most_tiles : 1);
+  };
+  p->tiles = tiles(kPrefixRows);
   p->prefix_splits = 0;
   p->tensor = 0;
   p->reach = 0x7fffffff;
@@ -1050,9 +1058,9 @@ void plan(const OasisSharedArgs* a, SharedParams* p) {
       // 32 / 8 heads of 128: 38.1 / 33.7, 49.8 / 34.2; 256 rows of 16 heads of 64: 53.8 / 56.1
       // behind 8192 tokens, 43.2 / 41.3 behind 2048; with own keys in ranges, up to 2048 of
       // them: 57.1 / 62.1.
-      const long long pairs = ((long long)group_rows * p->per + 255) / 256;
+      const long long pairs = tiles(256);
       p->tiles = (int)pairs;
-      p->reach = pairs * 256 < 0x7fffffff ? (int)pairs * 256 : 0x7fffffff;
+      p->reach = (int)(pairs * 256 < 0x7fffffff ? pairs * 256 : 0x7fffffff);
       const long long blocks = (long long)a->groups * K * pairs;
       long long n = sms / blocks;
       if (p->own_splits == 1 && n >= 6) n = n * 2 / 3;
@@ -1136,6 +1144,8 @@ int check_shared(const OasisSharedArgs* a) {
   OASIS_REQUIRE(a->heads >= c->kv_heads && a->heads <= 1024 && a->heads % c->kv_heads == 0,
                 "attention_shared: heads=%d kv_heads=%d", a->heads, c->kv_heads);
   OASIS_REQUIRE(a->rows >= 0 && a->groups >= 0, "attention_shared: rows=%d groups=%d", a->rows, a->groups);
+  OASIS_REQUIRE((long long)a->rows * c->kv_heads * ((a->heads / c->kv_heads + 7) / 8) < (1LL << 31),
+                "attention_shared: %d rows of %d heads are too many", a->rows, a->heads);
   OASIS_REQUIRE(a->scale > 0.f && a->scale <= 3e38f, "attention_shared: scale=%g", (double)a->scale);
   return OASIS_OK;
 }
@@ -1170,7 +1180,7 @@ int oasis_attention_shared(const OasisSharedArgs* a, oasis_stream_t stream) {
                   "attention_shared: stride %lld is not a positive multiple of 8 elements", s);
   SharedParams p;
   plan(a, &p);
-  const long long blocks = (long long)a->groups * c->kv_heads * (p.prefix_splits ? p.prefix_splits : 1) * p.tiles;
+  const long long blocks = (long long)p.groups * c->kv_heads * p.prefix_splits * p.tiles;
   const long long items = (long long)a->rows * c->kv_heads * p.head_tiles * p.own_splits;
   OASIS_REQUIRE(blocks < (1LL << 31) && items < (1LL << 31), "attention_shared: %d rows of %d heads are too many",
                 a->rows, a->heads);

@@ -7,6 +7,7 @@ import math
 import os
 import random
 import subprocess
+import sys
 import tempfile
 
 import pytest
@@ -597,3 +598,58 @@ def test_a_score_of_nan_alone_in_a_range(way, dim, at):
     got = run(way, q, c, 0, seqs, plan)
     assert bool(torch.isnan(got[:2]).all())
     check(got, q, c, 0, seqs, rows=[2])
+
+
+@pytest.mark.parametrize("hints", [
+    dict(group_rows_hint=1 << 30, prefix_pages_hint=15), dict(group_rows_hint=(1 << 31) - 1, prefix_pages_hint=15),
+    dict(group_rows_hint=1 << 30, prefix_pages_hint=1000), dict(group_rows_hint=(1 << 31) - 1, prefix_pages_hint=1000),
+])
+def test_a_group_hint_beyond_the_batch_is_the_batch(hints):
+    """A group has no more rows than the batch, whatever the hint: the same workspace, and no
+    count that overflows. In a process of its own, which a division by zero would end."""
+    code = f'''
+import ctypes as C, sys
+sys.path.insert(0, {ROOT!r})
+import __graft_entry__
+__graft_entry__.load_package()
+from tests.test_attention_shared import _args
+from oasis_b200 import _lib
+lib, sizes = _lib.load(), []
+for heads in (256, 128, 3):
+    for rows in (2000, 1 << 22):
+        for hint in ({hints["group_rows_hint"]}, rows):
+            a, keep = _args(dict(width=4096), rows=rows, heads=heads, groups=2, group_start=16, prefix_pages=16,
+                            group_rows_hint=hint, prefix_pages_hint={hints["prefix_pages_hint"]}, own_tokens_hint=5000)
+            sizes.append(lib.oasis_attention_shared_workspace_size(C.byref(a)))
+            a.workspace, a.workspace_bytes = 16, 8  # too small: refused before anything is launched
+            sizes[-1] = sizes[-1], lib.oasis_attention_shared(C.byref(a), None), lib.oasis_last_error()
+print(sizes[0::2] == sizes[1::2], all(x[0] > 8 and x[1] == -3 for x in sizes))
+'''
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True)
+    assert run.returncode == 0 and run.stdout.split() == ["True", "True"], (run.returncode, run.stdout, run.stderr[-500:])
+
+
+@pytest.mark.parametrize("kw,rc,text", [
+    (dict(rows=(1 << 31) - 1, heads=1024), -1, b"too many"),
+    (dict(rows=1 << 20, heads=1024, groups=1 << 19), -3, b"workspace"),  # mostly empty groups
+    (dict(rows=1 << 20, heads=1024, groups=3, group_rows_hint=-5), -3, b"workspace"),
+])
+def test_batches_of_any_size_are_launched_or_refused(kw, rc, text):
+    """The most rows, heads and groups that the arguments hold overflow no count."""
+    lib = _lib.load()
+    rest = dict(groups=1, group_start=16, prefix_pages=16, group_rows_hint=(1 << 31) - 1, prefix_pages_hint=15,
+                own_tokens_hint=5000, workspace=16, workspace_bytes=8)
+    a, _ = _args(dict(width=4096), **{**rest, **kw})
+    assert lib.oasis_attention_shared(C.byref(a), None) == rc and text in lib.oasis_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", WAYS)
+def test_the_largest_group_hint(way):
+    c, seqs, plan, g = build([(15, [250, 300, 241]), (20, [330, 400])], 16, 2, 64, BF16)
+    q = queries(5, 16, 64, BF16, g)
+    want = run(way, q, c, 0, seqs, plan)
+    check(want, q, c, 0, seqs)
+    plan.most_rows = (1 << 31) - 1
+    got = run(way, q, c, 0, seqs, plan)
+    check(got, q, c, 0, seqs)
