@@ -487,7 +487,8 @@ int oasis_pages_write(const OasisPageCache* cache, int layer, const void* k, con
                       const int* cu, const int* start, int n, int rows, oasis_stream_t stream);
 /* Makes the empty sequences dst[i] continue src[i] (as src[i] was when the call
  * began): whole pages are shared, the filled rows of a partial last page are copied
- * into a page of its own. deep != 0 copies every page. */
+ * into a page of its own. deep != 0 copies every page. A source's table entry outside
+ * the pool (BAD_PAGE) becomes the target's entry. */
 int oasis_pages_fork(const OasisPageCache* cache, const int* src, const int* dst, int n, int deep,
                      oasis_stream_t stream);
 /* Empties the sequences: their pages' counts fall by one. One that is empty

@@ -249,7 +249,9 @@ __device__ __forceinline__ int copy_parts(const PageArgs& c, int pages) {
 }
 
 // After plan_kernel<true>: the targets' table rows, the shared pages' counts and
-// the copies. Sources are not targets of the same call unless they were empty.
+// the copies. Sources are not targets of the same call unless they were empty. A source's
+// entry outside the pool is the target's too, and the page that was meant for its copy is
+// free again: there is nothing to copy, and what the page holds is not the sequence's.
 __global__ void __launch_bounds__(kCopyThreads) fork_kernel(PageArgs c, const int* __restrict__ src,
                                                             const int* __restrict__ dst, int n, int deep) {
   pdl_trigger();
@@ -263,15 +265,17 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(PageArgs c, const in
     int* to = c.table + (long long)dst[i] * W;
     const int whole = deep ? 0 : L / P, last = (int)pages_of(L, P);
     for (int k = threadIdx.x; k < last; k += kCopyThreads) {
-      int page;
+      int page = from[k];
+      const bool ok = page_ok(page, c.g.pages);
+      if (!ok) atomicOr(c.status, OASIS_PAGES_BAD_PAGE);
       if (k < whole) {
-        page = from[k];
-        if (page_ok(page, c.g.pages))
-          atomicAdd(&c.refs[page], 1);
-        else
-          atomicOr(c.status, OASIS_PAGES_BAD_PAGE);
+        if (ok) atomicAdd(&c.refs[page], 1);
       } else {
-        page = list[base[i] + k - whole];
+        const int own = list[base[i] + k - whole];
+        if (ok)
+          page = own;
+        else
+          c.refs[own] = 0;
       }
       to[k] = page;
     }
@@ -286,10 +290,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_kernel(PageArgs c, const in
     const int at = (deep ? 0 : L / P) + k - base[i];
     if (at >= W) continue;
     const int from = c.table[(long long)src[i] * W + at];
-    if (!page_ok(from, c.g.pages)) {
-      if (threadIdx.x == 0) atomicOr(c.status, OASIS_PAGES_BAD_PAGE);
-      continue;
-    }
+    if (!page_ok(from, c.g.pages)) continue;
     copy_page(c, from, list[k], min(P, L - at * P), (int)(u - (long long)k * parts), parts);
   }
 }

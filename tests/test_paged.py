@@ -381,3 +381,45 @@ def test_python_checks():
         c.write(2, rows, rows, ints([0]), ints([0, 3]), start)
     with pytest.raises(_lib.OasisError, match="n=9"):
         c.free(ints(list(range(9))))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("deep", [False, True])
+def test_a_fork_of_a_page_outside_the_pool(deep):
+    """What the source does not have its fork does not have either: the entry outside the pool
+    is the fork's too, no page of the pool stands in its place, and the pages meant for it are
+    free. A whole page and the partial last one, which every fork copies."""
+    c, o = make(pages=12, slots=4, width=4, layers=1)
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    extend(c, o, [0], [40], gen)
+    pages = c.table[0, :3].tolist()
+    c.table[0, 2] = 99
+    if deep:
+        c.table[0, 0] = -3
+    bad = [x for x in c.table[0, :3].tolist()]
+    c.fork(ints([0]), ints([1]), deep=deep)
+    torch.cuda.synchronize()
+    assert int(c.status.item()) == paged.BAD_PAGE
+    got = c.table[1, :3].tolist()
+    assert c.lengths.tolist() == [40, 40, 0, 0] and got[2] == 99
+    refs = [0] * 12
+    for p in pages:
+        refs[p] = 1
+    if deep:
+        assert got[0] == -3 and got[1] not in pages
+        refs[got[1]] = 1
+        assert torch.equal(c.pool[got[1]], c.pool[bad[1]])
+    else:
+        assert got[:2] == bad[:2]
+        refs[bad[0]], refs[bad[1]] = 2, 2
+    assert c.refs.tolist() == refs
+    q = torch.empty(2, 3, 64, dtype=c.dtype, device=DEV).normal_(generator=gen)
+    q[1] = q[0]
+    plan = paged.SharedPlan([], [], 40, DEV)
+    a = paged.attention_shared(q, c, 0, ints([0, 1]), plan)
+    assert torch.equal(a[0], a[1]) and bool(torch.isfinite(a).all())
+    c.free(ints([1]))
+    left = [0] * 12
+    for p in pages:
+        left[p] = 1
+    assert c.refs.tolist() == left
