@@ -122,7 +122,8 @@ class PagedCache:
     [sequences, max_pages], lengths [sequences] and page counts [pages].
 
     `from_tensors` builds the handle around existing tensors (a cache restored from
-    a checkpoint, or shared with other code)."""
+    a checkpoint, or shared with other code; `status` [1] too where its bits are to be
+    kept)."""
 
     def __init__(self, pages: int, page_size: int, layers: int, kv_heads: int, head_dim: int, sequences: int,
                  max_pages: int, dtype=torch.bfloat16, device="cuda"):
@@ -133,12 +134,12 @@ class PagedCache:
 
     @classmethod
     def from_tensors(cls, pool: torch.Tensor, table: torch.Tensor, lengths: torch.Tensor,
-                     refs: torch.Tensor) -> "PagedCache":
+                     refs: torch.Tensor, status: torch.Tensor | None = None) -> "PagedCache":
         self = cls.__new__(cls)
-        self._bind(pool, table, lengths, refs)
+        self._bind(pool, table, lengths, refs, status)
         return self
 
-    def _bind(self, pool, table, lengths, refs):
+    def _bind(self, pool, table, lengths, refs, status=None):
         if pool.dim() != 6 or pool.shape[2] != 2 or not pool.is_contiguous():
             raise ValueError("pool must be contiguous [pages, layers, 2, kv_heads, page_size, head_dim]")
         if pool.dtype not in DTYPES:
@@ -151,11 +152,13 @@ class PagedCache:
         _ints(table, "table", index, table.numel())
         _ints(lengths, "lengths", index, table.shape[0])
         _ints(refs, "refs", index, pool.shape[0])
-        self.pool, self.table, self.lengths, self.refs = pool, table, lengths, refs
+        if status is None:
+            status = torch.zeros(1, dtype=torch.int32, device=pool.device)
+        _ints(status, "status", index, 1)
+        self.pool, self.table, self.lengths, self.refs, self.status = pool, table, lengths, refs, status
         self.pages, self.layers, _, self.kv_heads, self.page_size, self.head_dim = pool.shape
         self.sequences, self.max_pages = table.shape
         self.dtype, self._index = pool.dtype, index
-        self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
         self.ws = workspace(_lib.load().oasis_pages_workspace_size(self.pages, self.sequences), self.device)
         c = _lib.OasisPageCache(pool.data_ptr(), self.pages, self.layers, self.kv_heads, self.page_size, self.head_dim,
                                 DTYPES[self.dtype], table.data_ptr(), self.sequences, self.max_pages, lengths.data_ptr(),
@@ -164,8 +167,9 @@ class PagedCache:
         self._at = C.cast(self._c, C.c_void_p).value
 
     def __reduce__(self):
-        """Copied and stored as its tensors: the struct holds their addresses."""
-        return PagedCache.from_tensors, (self.pool, self.table, self.lengths, self.refs)
+        """Copied and stored as its tensors: the struct holds their addresses. What has been
+        refused since the last `check` is among them."""
+        return PagedCache.from_tensors, (self.pool, self.table, self.lengths, self.refs, self.status)
 
     def reserve(self, seqs: torch.Tensor, cu: torch.Tensor, stream=None) -> torch.Tensor:
         """Room for cu[i + 1] - cu[i] more tokens behind sequence seqs[i]; returns

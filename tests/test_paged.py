@@ -423,3 +423,26 @@ def test_a_fork_of_a_page_outside_the_pool(deep):
     for p in pages:
         left[p] = 1
     assert c.refs.tolist() == left
+
+
+@pytest.mark.gpu
+def test_copies_and_stored_caches_keep_what_was_refused():
+    """A copy of a cache, or one stored and loaded, raises what the cache has been refused
+    since its last check; a handle on the same tensors shares the word."""
+    c = paged.PagedCache(1, 16, 1, 1, 64, 2, 4, device=DEV)
+    c.reserve(ints([0]), ints([0, 20]))  # two pages of one
+    buffer = io.BytesIO()
+    torch.save(c, buffer)
+    buffer.seek(0)
+    for other in (copy.deepcopy(c), torch.load(buffer, weights_only=False)):
+        with pytest.raises(_lib.OasisError, match="no free page"):
+            other.check()
+        other.check()
+    same = copy.copy(c)
+    with pytest.raises(_lib.OasisError, match="no free page"):
+        same.check()
+    c.check()
+    fresh = paged.PagedCache.from_tensors(c.pool, c.table, c.lengths, c.refs)
+    assert int(fresh.status.item()) == 0
+    with pytest.raises(ValueError, match="status must hold 1"):
+        paged.PagedCache.from_tensors(c.pool, c.table, c.lengths, c.refs, c.lengths)
