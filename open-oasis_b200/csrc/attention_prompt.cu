@@ -246,13 +246,13 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
     if (((r < 8 ? bad_a : bad_b) >> ((r & 7) * 4) & 0xf) == 0) continue;
     const int row = r0 + wr + r, lo = first[wr + r];
     if (lo > row) continue;
-    float acc[D / 32] = {}, m = -INFINITY, l = 0.f;
+    float acc[D / 32];
     row_by_keys<T, D>(
         q + row * p.q_row, p.scale_log2, row - lo + 1, [&](long long x) { return k + (lo + x) * p.k_row; },
-        [&](long long x) { return v + (lo + x) * p.v_row; }, acc, m, l);
+        [&](long long x) { return v + (lo + x) * p.v_row; }, acc);
 #pragma unroll
     for (int d = 0; d < D / 32; d += 2)
-      *reinterpret_cast<uint32_t*>(out + row * p.o_row + lane * (D / 32) + d) = E::pack(acc[d] / l, acc[d + 1] / l);
+      *reinterpret_cast<uint32_t*>(out + row * p.o_row + lane * (D / 32) + d) = E::pack(acc[d], acc[d + 1]);
   }
 }
 

@@ -400,16 +400,16 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int r = __ffs(bad) - 1;
         bad &= bad - 1;
         const int at = u.r0[t] + quarter * 32 + r, from = __shfl_sync(0xffffffffu, lo, r);
-        float acc[D / 32] = {}, rm = -INFINITY, rl = 0.f;
+        float acc[D / 32];
         __syncwarp();  // the row's first result is written
         row_by_keys<T, D>(
             static_cast<const T*>(p.q) + u.head[t] * p.q_head + at * p.q_row, sc, at - from + 1,
             [&](long long x) { return k0 + (from + x) * p.k_row; }, [&](long long x) { return v0 + (from + x) * p.v_row; },
-            acc, rm, rl);
+            acc);
         T* o = static_cast<T*>(p.out) + u.head[t] * p.o_head + at * p.o_row;
 #pragma unroll
         for (int d = 0; d < D / 32; d += 2)
-          *reinterpret_cast<uint32_t*>(o + lane * (D / 32) + d) = E::pack(acc[d] / rl, acc[d + 1] / rl);
+          *reinterpret_cast<uint32_t*>(o + lane * (D / 32) + d) = E::pack(acc[d], acc[d + 1]);
       }
     }
   }

@@ -88,19 +88,23 @@ __device__ __forceinline__ bool finite_f(float x) { return fabsf(x) <= 3.4028234
 // [lane DV, lane DV + DV)). `key(j)` and `val(j)` give lane-independent row pointers
 // of the j-th visible key or null for one to skip. The tiled kernels multiply a
 // masked probability of zero with whatever the masked value row holds, which is
-// wrong where that is an infinity or NaN; rows whose result is not finite are done
-// again here, where only visible keys take part. Returns whether any key did.
+// wrong where that is an infinity or NaN, and their sum of values is divided only at the
+// end, so that it overflows where values are near bf16's largest; rows whose result is not
+// finite are done again here, where only visible keys take part and o is the weighted mean
+// of the keys so far: never larger than they are. Zeros without a key; NaN where keys
+// score -inf all of them, as the formula's 0 / 0.
 template <typename T, int D, typename Key, typename Val>
-__device__ __noinline__ bool row_by_keys(const T* q, float scale_log2, long long keys, Key key, Val val,
-                                         float (&o)[D / 32], float& m, float& l) {
+__device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long keys, Key key, Val val,
+                                         float (&o)[D / 32]) {
   constexpr int DV = D / 32;
   const int lane = threadIdx.x & 31;
-  float qv[DV];
+  float qv[DV], m = -INFINITY, l = 0.f;
 #pragma unroll
   for (int d = 0; d < DV; d += 2) {
     const float2 x = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(q + lane * DV + d));
     qv[d] = x.x;
     qv[d + 1] = x.y;
+    o[d] = o[d + 1] = 0.f;
   }
   bool any = false;
   for (long long j = 0; j < keys; ++j) {
@@ -117,18 +121,21 @@ __device__ __noinline__ bool row_by_keys(const T* q, float scale_log2, long long
     for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
     s *= scale_log2;
     const float mn = (s != s) ? s : fmaxf(m, s);  // a NaN score makes the row NaN
-    const float sh = softmax_shift(mn), a = exp2f(m - sh), p = exp2f(s - sh);
+    const float sh = softmax_shift(mn), a = l * exp2f(m - sh), p = exp2f(s - sh);
     const T* vp = val(j);
-    l = l * a + p;
+    m = mn;
+    l = a + p;
+    const float keep = l == 0.f ? 1.f : a / l, add = l == 0.f ? 0.f : p / l;  // 0: no score above -inf yet
 #pragma unroll
     for (int d = 0; d < DV; d += 2) {
       const float2 x = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(vp + lane * DV + d));
-      o[d] = o[d] * a + p * x.x;
-      o[d + 1] = o[d + 1] * a + p * x.y;
+      o[d] = o[d] * keep + add * x.x;
+      o[d + 1] = o[d + 1] * keep + add * x.y;
     }
-    m = mn;
   }
-  return any;
+  if (any && l == 0.f)
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] = __int_as_float(0x7fffffff);
 }
 
 }  // namespace oasis

@@ -376,7 +376,8 @@ __device__ __forceinline__ void column_step(Columns<D>& c, const uint8_t* sk, co
 }
 
 // A row's result where the joined ranges are not finite: key by key, so that masked
-// places and the formula's own NaN come out as they should. Whole warp.
+// places, sums that overflow and the formula's own NaN come out as they should; zeros where
+// no page of it lies in the pool. Whole warp.
 template <typename T, int D>
 __device__ __noinline__ void row_again(const SharedParams& p, int b, int h) {
   int s;
@@ -389,15 +390,13 @@ __device__ __noinline__ void row_again(const SharedParams& p, int b, int h) {
     if (!page_ok(page, p.g.pages)) return nullptr;
     return pool + (tile_offset(p.g, page, p.layer, which, kvh) + (j % P) * (D / 8)) * 8;
   };
-  float acc[D / 32] = {}, m = -INFINITY, l = 0.f;
-  const bool any = row_by_keys<T, D>(
-      static_cast<const T*>(p.q) + b * p.q_row + h * p.q_head, p.scale_log2, len,
-      [&](long long j) { return at(j, 0); }, [&](long long j) { return at(j, 1); }, acc, m, l);
-  if (!any) l = 1.f;  // no page of it lies in the pool: zeros
+  float acc[D / 32];
+  row_by_keys<T, D>(static_cast<const T*>(p.q) + b * p.q_row + h * p.q_head, p.scale_log2, len,
+                    [&](long long j) { return at(j, 0); }, [&](long long j) { return at(j, 1); }, acc);
   T* out = static_cast<T*>(p.out) + b * p.o_row + h * p.o_head;
 #pragma unroll
   for (int d = 0; d < D / 32; d += 2)
-    *reinterpret_cast<uint32_t*>(out + lane * (D / 32) + d) = Elem<T>::pack(acc[d] / l, acc[d + 1] / l);
+    *reinterpret_cast<uint32_t*>(out + lane * (D / 32) + d) = Elem<T>::pack(acc[d], acc[d + 1]);
 }
 
 template <typename T, int D>

@@ -459,3 +459,31 @@ def test_blocks_of_one_tile(dim, begin, lengths, extra):
     check(out, q, k, v, cu)
     assert bool((out[:begin] == 7).all()) and bool((out[cu[-1] :] == 7).all())
     assert _lib.load().oasis_device_error(0) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_whose_sum_overflows(hint, dim):
+    """Values near the type's largest: their weighted mean is finite, their sum is not."""
+    lengths = [140, 3, 60]
+    q, k, v = inputs(lengths, 2, 1, dim, BF16, seed=18)
+    v.uniform_(1e38, 3e38, generator=torch.Generator(device=DEV).manual_seed(19))
+    v[:, :, 1::2] *= -1
+    cu = starts(lengths)
+    check(paged.attention_prompt(q, k, v, ints(cu), hint), q, k, v, cu)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_of_keys_that_weigh_nothing(hint, dim):
+    """Keys that a row sees and that score thousands below its others: whatever finite value
+    they have, none of it is in the result."""
+    q, k, v = inputs([300], 2, 1, dim, BF16, seed=21)
+    q[:, :, 0] = 1
+    k[:, :, 0] = 0
+    low = torch.arange(300, device=DEV) % 3 == 1
+    k[low, :, 0], v[low] = -3e4, 3e38
+    got = paged.attention_prompt(q, k, v, ints([0, 300]), hint)
+    check(got, q, k, v, [0, 300])

@@ -653,3 +653,30 @@ def test_the_largest_group_hint(way):
     plan.most_rows = (1 << 31) - 1
     got = run(way, q, c, 0, seqs, plan)
     check(got, q, c, 0, seqs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_values_whose_sum_overflows(way, dim):
+    """Values near the type's largest: their weighted mean is finite, their sum is not."""
+    c, seqs, plan, g = build([(15, [250, 100, 0, 17, 241]), (0, [7, 1])], 16, 2, dim, BF16)
+    c.pool[:, :, 1].uniform_(1e38, 3e38, generator=g)
+    c.pool[:, :, 1, :, :, 1::2] *= -1
+    q = queries(len(seqs), 4, dim, BF16, g)
+    check(run(way, q, c, 0, seqs, plan), q, c, 0, seqs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("way", WAYS)
+def test_values_of_keys_that_weigh_nothing(way, dim):
+    """Keys that a row sees and that score thousands below its others: whatever finite value
+    they have, none of it is in the result."""
+    c, seqs, plan, g = build([(15, [250, 300, 0, 17, 241]), (0, [40])], 16, 2, dim, BF16)
+    q = queries(len(seqs), 4, dim, BF16, g)
+    q[:, :, 0] = 1
+    c.pool[:, :, 0, :, :, 0] = 0
+    c.pool[:, :, 0, :, 1::3, 0] = -3e4
+    c.pool[:, :, 1, :, 1::3] = 3e38
+    check(run(way, q, c, 0, seqs, plan), q, c, 0, seqs)
