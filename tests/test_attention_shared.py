@@ -2,6 +2,7 @@
 against fp64 within the bound of its roundings; then the operators in a run."""
 from __future__ import annotations
 
+import copy
 import ctypes as C
 import math
 import os
@@ -680,3 +681,43 @@ def test_values_of_keys_that_weigh_nothing(way, dim):
     c.pool[:, :, 0, :, 1::3, 0] = -3e4
     c.pool[:, :, 1, :, 1::3] = 3e38
     check(run(way, q, c, 0, seqs, plan), q, c, 0, seqs)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name,pages,longest", [
+    ("alone", 0, 400), ("alone in ranges", 0, 1 << 14), ("tensor memory", 1 << 16, 300), ("tensor memory in ranges", 1 << 11, 1 << 16),
+    ("mma", 15, 300), ("mma in ranges", 15, 1 << 14),
+])
+def test_steps_without_a_pause(name, pages, longest):
+    """Decoding steps queued one behind the other, kernels of a step starting while the last
+    one ends, leave the bits of the same steps with a wait between all calls."""
+    rows, kv, steps = 40, 16, 60
+    g = torch.Generator(device=DEV).manual_seed(8)
+    c = paged.PagedCache(400, 16, 1, kv, 64, rows, 24, device=DEV)
+    new = torch.empty(250, 2 * kv, 64, dtype=BF16, device=DEV).normal_(generator=g)
+    start = c.reserve(ints([0]), ints([0, 250]))
+    c.write(0, new[:, :kv], new[:, kv:], ints([0]), ints([0, 250]), start)
+    c.fork(ints([0] * (rows - 1)), ints(list(range(1, rows))))
+    seqs, one = ints(list(range(rows))), ints(list(range(rows + 1)))
+    plan = paged.SharedPlan([rows], [15], longest, DEV)
+    plan.most_pages = pages
+    qkv = torch.empty(steps, rows, 3 * kv, 64, dtype=BF16, device=DEV).normal_(generator=g)
+
+    def go(cache, wait):
+        outs = []
+        for x in qkv:
+            at = cache.reserve(seqs, one)
+            wait()
+            cache.write(0, x[:, kv : 2 * kv], x[:, 2 * kv :], seqs, one, at)
+            wait()
+            outs.append(paged.attention_shared(x[:, :kv], cache, 0, seqs, plan))
+            wait()
+        return torch.stack(outs)
+
+    other = copy.deepcopy(c)
+    torch.cuda.synchronize()
+    quick = go(c, lambda: None)
+    slow = go(other, torch.cuda.synchronize)
+    assert torch.equal(quick, slow)
+    check(quick[-1], qkv[-1, :, :kv], c, 0, list(range(rows)))
+    c.check()
