@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
   uint8_t* const sv = sk + K_BYTES;
   // A thread's 16-byte chunks lie STEP rows apart, in the same swizzled column.
   constexpr int STEP = kRowsThreads / CH;
-  static_assert(STEP % 8 == 0 && kRowsTile % STEP == 0 && kRowsKeys % STEP == 0, "chunks of a thread");
+  static_assert(16 % STEP == 0 && STEP % 8 == 0 && kRowsTile % STEP == 0 && kRowsKeys % STEP == 0, "chunks of a thread");
   const int tr = tid / CH, tc = tid % CH;
   {
     const T* from = q + (long long)(r0 + tr) * p.q_row + tc * 8;
@@ -97,6 +97,17 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
   if (r0 >= end) {
     cp_async_wait_all();
     return;
+  }
+  // Rows behind the last sequence hold anything: their values become zeros, like their
+  // probabilities, since an infinity or NaN there would send the tile's rows to the repair.
+  // A row of a sequence meets those of its own 16 keys only.
+  if (r0 + kRowsTile > end) {
+    cp_async_wait_all();
+#pragma unroll
+    for (int i = 0; i < 16 / STEP; ++i) {
+      const int row = kRowsBefore + (end - r0) / 16 * 16 + i * STEP + tr;
+      if (r0 - kRowsBefore + row >= end) *reinterpret_cast<uint4*>(sv + tile_at<D>(row, tc)) = make_uint4(0, 0, 0, 0);
+    }
   }
   // The first row's sequence, a warp probing 32 places at a time; the other rows of the
   // tile belong to it or to the ones behind it.

@@ -211,6 +211,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tc_commit(&pv_done[t]);
         }
       };
+      // Rows of V block j behind the last sequence hold anything: zeros instead, like their
+      // probabilities, since an infinity or NaN there would send the tile's rows to the
+      // repair. It is the unit's last block, so that its stage is not loaded again; with two
+      // warps both write the same zeros, each ahead of its own products.
+      auto clear = [&](int j) {
+        const int row = max(0, end - (u.begin + j * kTile));
+        uint8_t* stage = sKV + (2 * j + 1) % C::STAGES * C::TILE_BYTES;
+        for (int c = 0; c < C::CHUNKS; ++c)
+          for (int i = row * 8 + lane; i < kTile * 8; i += 32)
+            *reinterpret_cast<uint4*>(stage + c * C::CHUNK_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();  // the products read V through the async proxy
+        __syncwarp();
+      };
       auto next_s = [&](int t, int j) {  // K block j has arrived
         if (!ok || !active(t, j)) return;
         if (j == first[t]) ok = wait_all(&q_full[t], 0, kDevTimeoutTmaFull);
@@ -228,6 +241,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           if (ok) release(2 * (j + 1));
         }
         ok = ok && arrived(2 * j + 1);
+        if (ok && u.begin + (j + 1) * kTile > end) clear(j);
         for (int t = t0; t < t1; ++t) {
           if (ok && active(t, j)) {
             ok = wait_all(&p_full[t], (j - first[t]) & 1, kDevTimeoutAccFull);

@@ -487,3 +487,22 @@ def test_values_of_keys_that_weigh_nothing(hint, dim):
     k[low, :, 0], v[low] = -3e4, 3e38
     got = paged.attention_prompt(q, k, v, ints([0, 300]), hint)
     check(got, q, k, v, [0, 300])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("heads,kv,dim,dtype", [(2, 1, 64, BF16), (3, 3, 64, FP16), (2, 1, 128, FP16), (3, 1, 128, BF16)])
+@pytest.mark.parametrize("lengths,extra", [([70], 1), ([140, 3, 90], 100), ([300], 15), ([129, 255], 300), ([64, 64, 128], 64)])
+def test_what_lies_behind_the_last_sequence_changes_no_bit(lengths, extra, heads, kv, dim, dtype, hint):
+    """NaN and infinities in padding rows leave every bit that zeros there leave: no row is
+    worked out another way because of them (which took hundreds of times as long)."""
+    q, k, v = inputs(lengths, heads, kv, dim, dtype, seed=22, extra=extra)
+    cu, n = ints(starts(lengths)), sum(lengths)
+    q[n:], k[n:], v[n:] = 0, 0, 0
+    want = paged.attention_prompt(q, k, v, cu, hint)
+    check(want, q, k, v, starts(lengths))
+    for bad in (math.nan, math.inf, -math.inf):
+        q[n:], k[n:], v[n:] = bad, bad, bad
+        out = torch.full_like(want, 7.0)
+        paged.attention_prompt(q, k, v, cu, hint, out=out)
+        assert torch.equal(out[:n], want[:n]) and bool((out[n:] == 7).all())
