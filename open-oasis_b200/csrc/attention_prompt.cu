@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
     const int row = r0 + wr + r, lo = first[wr + r];
     if (lo > row) continue;
     float acc[D / 32];
-    row_by_keys<T, D>(
+    row_by_keys<T, D, 2>(
         q + row * p.q_row, p.scale_log2, row - lo + 1, [&](long long x) { return k + (lo + x) * p.k_row; },
         [&](long long x) { return v + (lo + x) * p.v_row; }, acc);
 #pragma unroll

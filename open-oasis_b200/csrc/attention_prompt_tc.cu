@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
         const int at = u.r0[t] + quarter * 32 + r, from = __shfl_sync(0xffffffffu, lo, r);
         float acc[D / 32];
         __syncwarp();  // the row's first result is written
-        row_by_keys<T, D>(
+        row_by_keys<T, D, 8>(
             static_cast<const T*>(p.q) + u.head[t] * p.q_head + at * p.q_row, sc, at - from + 1,
             [&](long long x) { return k0 + (from + x) * p.k_row; }, [&](long long x) { return v0 + (from + x) * p.v_row; },
             acc);

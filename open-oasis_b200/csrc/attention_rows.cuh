@@ -84,19 +84,24 @@ __device__ __forceinline__ float softmax_shift(float m) { return m == -INFINITY 
 
 __device__ __forceinline__ bool finite_f(float x) { return fabsf(x) <= 3.402823466e38f; }
 
-// One query row of D = 32 DV dims, key by key, by a whole warp (lane holds dims
-// [lane DV, lane DV + DV)). `key(j)` and `val(j)` give lane-independent row pointers
-// of the j-th visible key or null for one to skip. The tiled kernels multiply a
-// masked probability of zero with whatever the masked value row holds, which is
-// wrong where that is an infinity or NaN, and their sum of values is divided only at the
-// end, so that it overflows where values are near bf16's largest; rows whose result is not
-// finite are done again here, where only visible keys take part and o is the weighted mean
-// of the keys so far: never larger than they are. Zeros without a key; NaN where keys
-// score -inf all of them, as the formula's 0 / 0.
-template <typename T, int D, typename Key, typename Val>
+// One query row of D = 32 DV dims by a whole warp (lane holds dims [lane DV, lane DV + DV)).
+// `key(j)` and `val(j)` give the row pointers of the j-th visible key or null for one to skip.
+// The tiled kernels multiply a masked probability of zero with whatever the masked value row
+// holds, which is wrong where that is an infinity or NaN, and their sum of values is divided
+// only at the end, so that it overflows where values are near bf16's largest; rows whose
+// result is not finite are done again here, where only visible keys take part and o is the
+// weighted mean of the keys so far: never larger than they are. Zeros without a key; NaN
+// where keys score -inf all of them, as the formula's 0 / 0, and from the first score of
+// NaN or +inf on, where every further sum is NaN.
+// 32 keys at a time, a lane for each one's score, BATCH 16-byte loads of a key and BATCH
+// value rows in flight (2 where the calling kernel has few registers): key by key through the
+// whole warp, each one's loads behind the shuffles of the one before, a row of 2000 keys
+// took 0.55 us a key.
+template <typename T, int D, int BATCH, typename Key, typename Val>
 __device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long keys, Key key, Val val,
                                          float (&o)[D / 32]) {
   constexpr int DV = D / 32;
+  const float nan = __int_as_float(0x7fffffff);
   const int lane = threadIdx.x & 31;
   float qv[DV], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -107,35 +112,77 @@ __device__ __noinline__ void row_by_keys(const T* q, float scale_log2, long long
     o[d] = o[d + 1] = 0.f;
   }
   bool any = false;
-  for (long long j = 0; j < keys; ++j) {
-    const T* kp = key(j);
-    if (!kp) continue;
+  for (long long j0 = 0; j0 < keys; j0 += 32) {
+    const long long j = j0 + lane;
+    const T *kp = nullptr, *vp = nullptr;
+    if (j < keys) kp = key(j), vp = val(j);
+    const unsigned there = __ballot_sync(0xffffffffu, kp != nullptr);
+    if (!there) continue;
     any = true;
     float s = 0.f;
+#pragma unroll 1
+    for (int c0 = 0; c0 < D / 8; c0 += BATCH) {
+      uint4 x[BATCH];
 #pragma unroll
-    for (int d = 0; d < DV; d += 2) {
-      const float2 x = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(kp + lane * DV + d));
-      s = fmaf(qv[d], x.x, fmaf(qv[d + 1], x.y, s));
+      for (int c = 0; c < BATCH; ++c)
+        x[c] = kp ? reinterpret_cast<const uint4*>(kp)[c0 + c] : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int c = 0; c < BATCH; ++c) {
+        const uint32_t w[4] = {x[c].x, x[c].y, x[c].z, x[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 y = Elem<T>::unpack(w[e]);
+          const int d = 2 * e % DV, from = ((c0 + c) * 8 + 2 * e) / DV;
+          s = fmaf(__shfl_sync(0xffffffffu, qv[d], from), y.x, s);
+          s = fmaf(__shfl_sync(0xffffffffu, qv[d + 1], from), y.y, s);
+        }
+      }
     }
+    s = kp ? s * scale_log2 : -INFINITY;
+    if (__any_sync(0xffffffffu, !(s < INFINITY))) {
 #pragma unroll
-    for (int w = 16; w; w >>= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
-    s *= scale_log2;
-    const float mn = (s != s) ? s : fmaxf(m, s);  // a NaN score makes the row NaN
+      for (int d = 0; d < DV; ++d) o[d] = nan;
+      return;
+    }
+    float mn = fmaxf(m, s);
+#pragma unroll
+    for (int w = 16; w; w >>= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, w));
     const float sh = softmax_shift(mn), a = l * exp2f(m - sh), p = exp2f(s - sh);
-    const T* vp = val(j);
-    m = mn;
-    l = a + p;
-    const float keep = l == 0.f ? 1.f : a / l, add = l == 0.f ? 0.f : p / l;  // 0: no score above -inf yet
+    float sum = p;
 #pragma unroll
-    for (int d = 0; d < DV; d += 2) {
-      const float2 x = Elem<T>::unpack(*reinterpret_cast<const uint32_t*>(vp + lane * DV + d));
-      o[d] = o[d] * keep + add * x.x;
-      o[d + 1] = o[d + 1] * keep + add * x.y;
+    for (int w = 16; w; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    m = mn;
+    l = a + sum;
+    // 0: no score above -inf yet; their weight is zero, which an infinite value makes NaN
+    const float keep = l == 0.f ? 1.f : a / l, weight = l == 0.f ? 0.f : p / l;
+#pragma unroll
+    for (int d = 0; d < DV; ++d) o[d] *= keep;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 32; i0 += BATCH) {
+      uint32_t y[BATCH][DV / 2];
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const T* v = reinterpret_cast<const T*>(
+            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vp), i0 + i));
+        const bool in = there >> (i0 + i) & 1;
+#pragma unroll
+        for (int d = 0; d < DV / 2; ++d) y[i][d] = in ? reinterpret_cast<const uint32_t*>(v + lane * DV)[d] : 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; ++i) {
+        const float f = __shfl_sync(0xffffffffu, weight, i0 + i);
+#pragma unroll
+        for (int d = 0; d < DV / 2; ++d) {
+          const float2 x = Elem<T>::unpack(y[i][d]);
+          o[2 * d] = fmaf(f, x.x, o[2 * d]);
+          o[2 * d + 1] = fmaf(f, x.y, o[2 * d + 1]);
+        }
+      }
     }
   }
   if (any && l == 0.f)
 #pragma unroll
-    for (int d = 0; d < DV; ++d) o[d] = __int_as_float(0x7fffffff);
+    for (int d = 0; d < DV; ++d) o[d] = nan;
 }
 
 }  // namespace oasis

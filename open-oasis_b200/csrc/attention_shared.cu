@@ -391,7 +391,7 @@ __device__ __noinline__ void row_again(const SharedParams& p, int b, int h) {
     return pool + (tile_offset(p.g, page, p.layer, which, kvh) + (j % P) * (D / 8)) * 8;
   };
   float acc[D / 32];
-  row_by_keys<T, D>(static_cast<const T*>(p.q) + b * p.q_row + h * p.q_head, p.scale_log2, len,
+  row_by_keys<T, D, 4>(static_cast<const T*>(p.q) + b * p.q_row + h * p.q_head, p.scale_log2, len,
                     [&](long long j) { return at(j, 0); }, [&](long long j) { return at(j, 1); }, acc);
   T* out = static_cast<T*>(p.out) + b * p.o_row + h * p.o_head;
 #pragma unroll

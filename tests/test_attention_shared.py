@@ -721,3 +721,32 @@ def test_steps_without_a_pause(name, pages, longest):
     assert torch.equal(quick, slow)
     check(quick[-1], qkv[-1, :, :kv], c, 0, list(range(rows)))
     c.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 48)])
+@pytest.mark.parametrize("way", WAYS)
+def test_a_sum_that_overflows_beside_pages_outside_the_pool(way, dim, page):
+    """Rows that are worked out again leave out what lies outside the pool, and one that has
+    nothing in it gives zeros."""
+    c, seqs, plan, g = build([(2, [5 * page + 3, 3 * page]), (0, [4 * page, page + 1, 70])], page, 2, dim, BF16)
+    c.pool[:, :, 1].uniform_(1e38, 3e38, generator=g)
+    q = queries(len(seqs), 4, dim, BF16, g)
+    c.table[seqs[0], 3] = -1
+    c.table[seqs[2], 0], c.table[seqs[2], 2] = 1 << 30, c.pages
+    c.table[seqs[3], :2] = ints([-1, -1])
+    got = run(way, q, c, 0, seqs, plan)
+    torch.cuda.synchronize()
+    assert int(c.status.item()) == paged.BAD_PAGE
+    table, lengths = c.table.tolist(), c.lengths.tolist()
+    for b, s in enumerate(seqs):
+        held = [(p, x) for t in range(lengths[s]) for p, x in [(table[s][t // page], t % page)] if 0 <= p < c.pages]
+        if not held:
+            assert b == 3 and not bool(got[b].any())
+            continue
+        pages, slots = (torch.tensor(x, device=DEV) for x in zip(*held))
+        kv = c.pool[pages, 0, :, :, slots]  # [tokens, 2, heads, dim]
+        want = O.attention_rows(q[b : b + 1], kv[:, 0], kv[:, 1])
+        reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * kv[:, 0].double().norm(dim=-1).max())
+        bound = O.error_bound(want, want, reach, len(held), dim, BF16)
+        assert bool(((got[b : b + 1].double() - want).abs() <= bound).all()), b
