@@ -194,8 +194,10 @@ __global__ void __launch_bounds__(kRowsThreads, D == 64 ? 6 : 3) prompt_rows_ker
       }
       na = fmaxf(na, ma);
       nb = fmaxf(nb, mb);
-      const float sa = softmax_shift(na), sb = softmax_shift(nb);
+      float sa = softmax_shift(na), sb = softmax_shift(nb);
       const float fa = ex2_approx(ma - sa), fb = ex2_approx(mb - sb);
+      sa -= kLift<T>;
+      sb -= kLift<T>;
       ma = na;
       mb = nb;
 #pragma unroll

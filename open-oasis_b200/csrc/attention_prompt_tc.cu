@@ -12,10 +12,11 @@
 //   O += P V         tcgen05.mma 128 x D x 128 accumulating in TMEM, V as it lies in
 //                    memory (MN-major B)
 // While one tile is in the softmax the other one's products run. The maximum m that is
-// subtracted is only raised when a row exceeds it by more than 2^8: P stays below 2^8,
-// the sum is exact to fp32 either way, and O in TMEM is rescaled a few times per row
-// instead of once per block. With D = 64 TMEM holds S, P and O of both tiles apart, so
-// the next S is computed during the softmax; with D = 128 P takes S's columns.
+// subtracted is only raised when a row exceeds it by more than 2^8 (fp16: 2^6): P stays below
+// 2^8 (fp16, where it is lifted besides: 2^15), the sum is exact to fp32 either way, and O in
+// TMEM is rescaled a few times per row instead of once per block. With D = 64 TMEM holds S, P
+// and O of both tiles apart, so the next S is computed during the softmax; with D = 128 P
+// takes S's columns.
 //
 // Warps 0-3 and 4-7: softmax and output of tile 0 and 1. Warp 8 loads Q, K and V by TMA
 // (128-byte swizzle, K and V blocks in one ring). Warps 9 and 10 (D = 128: 9 alone) issue
@@ -330,7 +331,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           pk[x * 16 + k / 2] = E::pack(y.x, y.y);  // the one rounding inside the sum, half a step per term
         }
       };
-      const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
+      const bool raise = bm > m + kRaise<T>;  // -inf + 8 is -inf: any finite score raises it
       const bool any_raise = __any_sync(0xffffffffu, raise);
       float alpha = 1.f;
       if (raise) {
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1)
           tmem_st32(o_at + x * 32, o);
         }
       };
-      const float shift = softmax_shift(m);
+      const float shift = softmax_shift(m) - kTileLift<T>;
 #pragma unroll
       for (int x = 0; x < 4; ++x) quarter_of_p(x, shift);
       const float2 part = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));

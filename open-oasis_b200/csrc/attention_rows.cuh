@@ -72,6 +72,14 @@ struct Elem<__half> {
   }
 };
 
+// Probabilities of the mma.sync kernels, and so their sums, are 2^kLift times those relative to
+// the running maximum. fp16's normal numbers end at 2^-14, and a weight below that is
+// rounded by more than half a step of its own: where one key outweighs the others by 14 to 16
+// nats, what those add was off by 17 to 67 half steps. 2^15 is the most that the type holds of
+// the largest weight; weights are whole down to 2^-29 of it. bf16 has fp32's exponents.
+template <typename T>
+constexpr float kLift = Elem<T>::kHalf ? 15.f : 0.f;
+
 // Byte offset of 16-byte chunk `chunk` of row `row` in a tile of D-element rows whose
 // chunks are XOR-swizzled by the row, so that eight rows' same chunk hits all banks.
 template <int D>

@@ -77,9 +77,11 @@ __device__ __forceinline__ void softmax_step(float (&x)[2][4], Running& r, float
   }
   na = fmaxf(na, r.ma);
   nb = fmaxf(nb, r.mb);
-  const float sa = softmax_shift(na), sb = softmax_shift(nb);
+  float sa = softmax_shift(na), sb = softmax_shift(nb);
   fa = ex2_approx(r.ma - sa);
   fb = ex2_approx(r.mb - sb);
+  sa -= kLift<T>;
+  sb -= kLift<T>;
   r.ma = na;
   r.mb = nb;
 #pragma unroll
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
       const int h = kvh * p.per + at.head_of(ra + half * 8);
       const long long slot = (b * p.heads + h) * splits + split;
       const float mm = half ? run.mb : run.ma, ll = half ? run.lb : run.la;
-      if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm, ll);
+      if ((lane & 3) == 0) p.part_ml[slot] = make_float2(mm - kLift<T>, ll);
       if (mm == -INFINITY && ll == 0.f) continue;  // nothing in this range: its sums are not read
 #pragma unroll
       for (int t = 0; t < NT; ++t)
@@ -349,8 +351,10 @@ __device__ __forceinline__ void column_step(Columns<D>& c, const uint8_t* sk, co
   }
   na = fmaxf(na, c.m[0]);
   nb = fmaxf(nb, c.m[1]);
-  const float sa = softmax_shift(na), sb = softmax_shift(nb);
+  float sa = softmax_shift(na), sb = softmax_shift(nb);
   const float fa = ex2_approx(c.m[0] - sa), fb = ex2_approx(c.m[1] - sb);
+  sa -= kLift<T>;
+  sb -= kLift<T>;
   c.m[0] = na;
   c.m[1] = nb;
   x[0] = ex2_approx(fmaf(x[0], scale_log2, -sa));
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     for (int half = 0; half < 2; ++half) {
       if (ca + half >= nh) continue;
       const long long slot = ((long long)b * p.heads + h0 + ca + half) * splits + p.prefix_splits + split;
-      if (dim == 0) p.part_ml[slot] = make_float2(run.m[half], run.l[half]);
+      if (dim == 0) p.part_ml[slot] = make_float2(run.m[half] - kLift<T>, run.l[half]);
       if (run.m[half] == -INFINITY && run.l[half] == 0.f) continue;  // its sums are not read
 #pragma unroll
       for (int t = 0; t < MT; ++t) {
@@ -563,7 +567,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
     pdl_wait();  // nobody ends before the prefix kernel does: what follows waits for this one alone
     return;
   }
-  // the prefix ranges of these heads join here
+  // the prefix ranges of these heads join here, each relative to its maximum less its lift
   pdl_wait();
   unsigned bad = 0;
   float inv[2];
@@ -571,7 +575,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32) shared_own_kernel(SharedParams
   for (int half = 0; half < 2; ++half) {
     const bool mine = ca + half < nh;
     const long long slot = ((long long)b * p.heads + h0 + (mine ? ca + half : 0)) * splits;
-    const float m = run.m[half];
+    const float m = run.m[half] - kLift<T>;
     float l = run.l[half];
     if (group >= 0 && mine) {
       // the joint maximum first, so that the ranges' loads do not wait for one another

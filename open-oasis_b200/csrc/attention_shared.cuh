@@ -16,7 +16,8 @@ struct SharedParams {
   const int *table, *lengths, *seqs, *group_start, *prefix_pages;
   int* status;
   float* part_o;   // [rows heads][splits][D]
-  float2* part_ml; // [rows heads][splits] (maximum, sum), maximum in base-2 exponents
+  float2* part_ml; // [rows heads][splits] (what sum and values are relative to, sum): base-2 exponent of
+                   // the maximum less the kernel's lift of its probabilities
   int rows, groups, heads, per, layer;  // per: heads of a key head
   int prefix_splits, own_splits, own_units, tiles, head_tiles, whole;  // own_units: of a split but the last
   int team;    // warps of an item of own keys: 1 or 4

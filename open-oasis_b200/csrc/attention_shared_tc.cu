@@ -366,7 +366,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           pk[x * 16 + k / 2] = E::pack(y.x, y.y);  // the one rounding inside the sum, half a step per term
         }
       };
-      const bool raise = bm > m + kRaise;  // -inf + 8 is -inf: any finite score raises it
+      const bool raise = bm > m + kRaise<T>;  // -inf + 8 is -inf: any finite score raises it
       const bool any_raise = __any_sync(0xffffffffu, raise);
       float alpha = 1.f;
       if (raise) {
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           tmem_st32(o_at + x * 32, o);
         }
       };
-      const float shift = softmax_shift(m);
+      const float shift = softmax_shift(m) - kTileLift<T>;
 #pragma unroll
       for (int x = 0; x < 4; ++x) quarter_of_p(x, shift);
       const float2 part = split2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])));
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
       // No score above -inf: the masked keys left at most 2^-136 each in the sum. Only a score of
       // NaN, which the maximum passes over, leaves more (or NaN), and then the row is NaN.
       if (m == -INFINITY) l = l < 1.f ? 0.f : __int_as_float(0x7fffffff);
-      if (mine) p.part_ml[slot_of(lane)] = make_float2(m, l);
+      if (mine) p.part_ml[slot_of(lane)] = make_float2(m - kTileLift<T>, l);
       // O through this tile's Q, which no product reads any more: 32 columns of 32 rows,
       // so that a store covers four rows' 128 bytes
       const unsigned mine_rows = __ballot_sync(0xffffffffu, mine && !(m == -INFINITY && l == 0.f));

@@ -6,7 +6,15 @@
 namespace oasis {
 
 constexpr int kTile = 128;  // query rows of a tile, keys of a block
-constexpr float kRaise = 8.f;  // base-2 exponents that a score may exceed the subtracted maximum by
+// Base-2 exponents that a score may exceed the subtracted maximum by, and those that P is
+// lifted by besides (see kLift): together 15 at most in fp16, where weights are whole down to
+// 2^-23 of the largest. A smaller margin rescales O more often: 3 with a lift of 12, 5 with 10,
+// 6 with 9 and 8 with 7 took 334.8 / 323.0 / 317.5 / 315.1 us for 6042 tokens in 4 sequences, 32 / 8
+// heads of 128.
+template <typename T>
+constexpr float kRaise = Elem<T>::kHalf ? 6.f : 8.f;
+template <typename T>
+constexpr float kTileLift = Elem<T>::kHalf ? 9.f : 0.f;
 
 // One word per translation unit, read by its own host function.
 static __device__ int g_wait_error = 0;
@@ -82,7 +90,7 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe, for x <= 8:
+// 2^x of two values on the FMA pipe, for x <= 15:
 // x = n + f with n the nearest whole number (Cody and Waite's reduction: adding
 // 1.5 2^23 leaves n in the low bits), 2^f on [-1/2, 1/2] by the polynomial of least
 // relative error (Remez), n added to the exponent field. Relative error 7.5e-5 in

@@ -530,3 +530,28 @@ def test_a_batch_of_nan_is_not_worked_out_key_by_key():
         t[:] = math.nan
     dirty, out = took()
     assert bool(torch.isnan(out).all()) and dirty < 40 * clean, (clean, dirty)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hint", [1, 1 << 20])
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, FP16), (64, BF16)])
+@pytest.mark.parametrize("nats", [10, 14, 15.5])
+def test_one_key_outweighs_the_others(nats, dim, dtype, hint):
+    """A first key that takes nearly all of the weight and has a value of zero: what the others,
+    `nats` below it, add is as exact as a probability's one rounding. The bound is the usual
+    one without its allowance for probabilities that underflow; half a subnormal step for
+    results among the type's subnormal numbers."""
+    n = 3000
+    g = torch.Generator(device=DEV).manual_seed(24)
+    q, k, v = (torch.zeros(n, 1, dim, dtype=dtype, device=DEV) for _ in range(3))
+    q[:, :, :2] = 1
+    k[1:, 0, 0] = -nats * dim ** 0.5
+    k[1:, 0, 1] = torch.empty(n - 1, device=DEV).uniform_(-2, 2, generator=g).to(dtype)
+    v[1:] = 1
+    got = paged.attention_prompt(q, k, v, ints([0, n]), hint)
+    want = O.attention_prompt(q, k, v, [0, n])
+    reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * k.double().norm(dim=-1).max())
+    allowed = 2.0 ** -24 * (1 + 2 * n) if dtype == FP16 else 2.0 ** -120
+    bound = O.error_bound(want, want, reach, n, dim, dtype) - allowed + 2.0 ** (-25 if dtype == FP16 else -120)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())

@@ -750,3 +750,29 @@ def test_a_sum_that_overflows_beside_pages_outside_the_pool(way, dim, page):
         reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * kv[:, 0].double().norm(dim=-1).max())
         bound = O.error_bound(want, want, reach, len(held), dim, BF16)
         assert bool(((got[b : b + 1].double() - want).abs() <= bound).all()), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,dtype", [(64, FP16), (128, FP16), (64, BF16)])
+@pytest.mark.parametrize("nats", [10, 14, 15.5])
+@pytest.mark.parametrize("way", WAYS)
+def test_one_key_outweighs_the_others(way, nats, dim, dtype):
+    """A first token that takes nearly all of the weight and has a value of zero: what the
+    others, `nats` below it, add is as exact as a probability's one rounding (the bound as for
+    packed prompts)."""
+    c, seqs, plan, g = build([(15, [250, 300, 1100, 241]), (0, [900, 70])], 16, 1, dim, dtype)
+    c.pool.zero_()
+    c.pool[:, :, 0, :, :, 0] = -nats * dim ** 0.5
+    c.pool[:, :, 0, :, :, 1] = torch.empty(c.pool.shape[:2] + c.pool.shape[3:5], device=DEV).uniform_(-2, 2, generator=g)
+    c.pool[:, :, 1] = 1
+    for s in seqs:
+        c.pool[int(c.table[s, 0]), :, :, :, 0] = 0
+    q = torch.zeros(len(seqs), 2, dim, dtype=dtype, device=DEV)
+    q[:, :, :2] = 1
+    got = run(way, q, c, 0, seqs, plan)
+    want = O.attention_cached(q, c.pool, c.table.tolist(), c.lengths.tolist(), 0, seqs)
+    reach = dim ** -0.5 * float(q.double().norm(dim=-1).max() * c.pool[:, 0, 0].double().norm(dim=-1).max())
+    allowed = 2.0 ** -24 * (1 + 2 * 1100) if dtype == FP16 else 2.0 ** -120
+    bound = O.error_bound(want, want, reach, 1100, dim, dtype) - allowed + 2.0 ** (-25 if dtype == FP16 else -120)
+    off = (got.double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
