@@ -10,8 +10,8 @@
 // prompt_rows_kernel: 64 query rows x one head per block, a warp per 16 rows, mma.sync
 // fragments with the running softmax in registers. For short sequences, where a tile
 // sees little more than its own rows and the least is reading q, k, v and writing o:
-// 37584 rows of 9216 sequences of 1 to 8 tokens, 16 heads of 64, 308 MB: 79 us (3.9 TB/s;
-// a copy of as many bytes 47 us). What is left is issue, 54 % of the cycles, and the
+// 37584 rows of 9216 sequences of 1 to 8 tokens, 16 heads of 64, 308 MB: 77 us (4.0 TB/s;
+// a copy of as many bytes 47 us). What is left is issue, 51 % of the cycles, and the
 // latency of a block's offsets and loads: six blocks an SM (D = 128: three) hide part of
 // it; seven or eight with fewer registers, and several heads per block with the next
 // one's loads ahead (115 us), were slower.

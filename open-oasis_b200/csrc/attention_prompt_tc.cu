@@ -25,11 +25,11 @@
 // Every wait is bounded and leaves a code in this file's error word.
 //
 // Bound: with D = 64 the exponentials (one per score, 16 per clock and SM) take twice
-// the tensor time, with D = 128 as long as it. 16384 tokens, 16 heads of 64: 703 us,
-// 782 TFLOP/s; 16 heads of 128: 1033 us, 1064 TFLOP/s; 6042 tokens in 4 sequences, 32 / 8
-// heads of 128: 267 us, 1104 TFLOP/s; 9216 tokens in 8 sequences, 16 heads of 64: 96 us
-// (clocks 1.55 to 1.97 GHz, the power cap the reason). With D = 64 a pair of tiles takes
-// about 2800 clocks a key block where the exponentials left to the special-function unit
+// the tensor time, with D = 128 as long as it. 16384 tokens, 16 heads of 64: 674 us,
+// 815 TFLOP/s; 16 heads of 128: 1005 us, 1094 TFLOP/s; 6042 tokens in 4 sequences, 32 / 8
+// heads of 128: 261 us, 1129 TFLOP/s (up to 316 us where the power cap holds the clock at 1.55
+// of 1.97 GHz); 9216 tokens in 8 sequences, 16 heads of 64: 94 us. With D = 64 a pair of tiles
+// takes about 2800 clocks a key block where the exponentials left to the special-function unit
 // take 1536: S's load, maximum, exponentials and P's store follow one another in a warp.
 // Measured slower: all exponentials on that unit, or 3 and 4 of 8 on the FMA pipe; a row
 // in two threads (16 softmax warps); the two tiles held half a block apart; P handed over

@@ -12,11 +12,11 @@
 // shared_own_kernel: each row's keys behind the prefix: four warps (or one) per (row, key
 // head, range), 16 keys a step, the heads of a key head as the eight columns of a fragment.
 // The least is reading the keys and values once: 32 rows of up to 4096 tokens, 32 / 8 heads
-// of 128, 97 MB: 38 us (2.5 TB/s) with the join; a block's lookups before its first load,
+// of 128, 97 MB: 29 us (3.4 TB/s) with the join; a block's lookups before its first load,
 // two steps of keys in flight per warp and the rows' different lengths are the rest. It
 // runs beside the prefix kernel. With one range it joins the prefix's and
 // writes the result; otherwise shared_join_kernel does, a warp per (row, head).
-// 64 rows behind 8192 shared tokens, up to 1024 own ones, 32 / 8 heads of 128: 49 us, about
+// 64 rows behind 8192 shared tokens, up to 1024 own ones, 32 / 8 heads of 128: 48 us, about
 // 25 for the prefix, the own keys beside and behind it and 8 to 10 for the join; the bytes
 // alone would take 10.
 // shared_whole_kernel: both in one pass where rows are many and short.

@@ -11,7 +11,7 @@
 // Bound: what is copied, read and written once (HBM), and for small calls the two
 // launches; the planning block reads refs up to the last page it hands out, and takes 6
 // to 7 us for its chain of searches and sums. Full copies of six sessions, 165 MB read
-// and written: 41 us (4.0 TB/s); 60 forks of four sessions, 49 MB: 23 us; 24 sessions
+// and written: 40 us (4.1 TB/s); 60 forks of four sessions, 49 MB: 23 us; 24 sessions
 // ended, compacted, reserved and written in four layers, twice, 356 MB: 108 us.
 #include <limits.h>
 

@@ -247,8 +247,9 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu: torc
 class SharedPlan:
     """Which rows of a batch share a prefix: group g is the next group_rows[g] rows, and
     the first prefix_pages[g] pages of their sequences are the same (PagedCache.fork
-    leaves them so). `longest`: the most tokens of a sequence in the calls to come (a
-    hint that chooses splits). Made once for a batch and kept while it lasts."""
+    leaves them so; it is not checked). `longest`: the most tokens of a sequence in the
+    calls to come (a hint that chooses splits). Made once for a batch and kept while it lasts:
+    a row that is freed and filled again, or replaced by a full copy, no longer shares."""
 
     def __init__(self, group_rows: list[int], prefix_pages: list[int], longest: int, device="cuda"):
         if len(group_rows) != len(prefix_pages) or any(r < 0 for r in group_rows) or any(p < 0 for p in prefix_pages):
