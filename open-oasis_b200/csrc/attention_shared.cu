@@ -222,9 +222,10 @@ __global__ void __launch_bounds__(kThreads) shared_prefix_kernel(SharedParams p)
         const int t = u * kUnit;
         const int page = u < u1 ? lead[t / P] : -1;
         const bool ok = page_ok(page, p.g.pages);
+        const bool in = ok && t + r % kUnit < common;  // rows behind the sequences hold anything: zero instead
         const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P + r % kUnit) * CH + c;
-        cp_async16(kd + tile_at<D>(r, c), pool + at, ok);
-        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + p.g.kv_heads * tile_vectors(p.g), ok);
+        cp_async16(kd + tile_at<D>(r, c), pool + at, in);
+        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + p.g.kv_heads * tile_vectors(p.g), in);
         if (c == 0 && r % kUnit == 0) {
           unit_ok[j & 1][r / kUnit] = ok;
           if (!ok && u < u1) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);
@@ -837,8 +838,9 @@ __global__ void __launch_bounds__(kThreads, D == 64 ? 6 : 3) shared_whole_kernel
         const int page = lead[t / P];
         const bool ok = page_ok(page, p.g.pages);
         const long long at = tile_offset(p.g, ok ? page : 0, p.layer, 0, kvh) + (long long)(t % P + r % kUnit) * CH + c;
-        cp_async16(kd + tile_at<D>(r, c), pool + at, ok);
-        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + to_v, ok);
+        const bool in = ok && t + r % kUnit < common;  // rows behind the sequences hold anything: zero instead
+        cp_async16(kd + tile_at<D>(r, c), pool + at, in);
+        cp_async16(kd + TILE + tile_at<D>(r, c), pool + at + to_v, in);
         if (c == 0 && r % kUnit == 0) {
           unit_ok[j & 1][r / kUnit] = ok;
           if (!ok) atomicOr(p.status, OASIS_PAGES_BAD_PAGE);

@@ -261,6 +261,19 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           tc_commit(&pv_done[t]);
         }
       };
+      // Rows of V block j behind the longest sequence, where that ends inside a box, hold
+      // anything: zeros instead, like their probabilities, since an infinity or NaN there would
+      // send every row to the repair. It is the prefix's last block, so that its stage is
+      // not loaded again; with two warps both write the same zeros, each ahead of its own products.
+      auto clear = [&](int j) {
+        const int row = common - (begin + j) * kTile;
+        uint8_t* stage = sKV + (2 * j + 1) % C::STAGES * C::TILE_BYTES;
+        for (int c = 0; c < C::CHUNKS; ++c)
+          for (int i = row * 8 + lane; i < kTile * 8; i += 32)
+            *reinterpret_cast<uint4*>(stage + c * C::CHUNK_BYTES + i * 16) = make_uint4(0, 0, 0, 0);
+        fence_proxy_async();  // the products read V through the async proxy
+        __syncwarp();
+      };
       auto next_s = [&](int t, int j) {  // K block j has arrived
         if (!ok || !active(t)) return;
         if (C::kApart && j > 0) ok = wait_all(&s_read[t], (j - 1) & 1, kDevTimeoutAccEmpty);
@@ -279,6 +292,7 @@ __global__ void __launch_bounds__(kSharedThreads, 1)
           if (ok) release(2 * (j + 1));
         }
         ok = ok && arrived(2 * j + 1);
+        if (ok && (begin + j + 1) * kTile > common && common % box_rows) clear(j);
         for (int t = t0; t < t1; ++t) {
           if (ok && active(t)) {
             ok = wait_all(&p_full[t], j & 1, kDevTimeoutAccFull);

@@ -776,3 +776,31 @@ def test_one_key_outweighs_the_others(way, nats, dim, dtype):
     bound = O.error_bound(want, want, reach, 1100, dim, dtype) - allowed + 2.0 ** (-25 if dtype == FP16 else -120)
     off = (got.double() - want).abs()
     assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("page", [16, 48, 256])
+@pytest.mark.parametrize("tokens", [150, 700])
+@pytest.mark.parametrize("dim,dtype", [(64, BF16), (128, FP16)])
+@pytest.mark.parametrize("way", WAYS)
+def test_what_lies_behind_the_sequences_changes_no_bit(way, dim, dtype, tokens, page):
+    """NaN and infinities behind the last token of a group's rows, also where all of them end
+    inside the named prefix, leave every bit that zeros there leave: no row is worked out
+    another way because of them."""
+    n = -(-tokens // page)
+    groups = [(n, [n * page - 7, n * page - 100, 0]), (n, [n * page + 5, n * page + 21]), (1, [9]), (0, [40, 3])]
+    c, seqs, plan, g = build(groups, page, 2, dim, dtype, layers=1)
+    q = queries(len(seqs), 6, dim, dtype, g)
+    lists, lengths = c.table.tolist(), c.lengths.tolist()
+    places = []
+    for b in (0, 3, 4, 5, 6, 7):
+        t = lengths[seqs[b]]
+        places += [(lists[seqs[b]][t // page], x) for x in range(t % page, page)]
+    pages, slots = (torch.tensor(x, device=DEV) for x in zip(*places))
+    c.pool[pages, :, :, :, slots] = 0
+    want = run(way, q, c, 0, seqs, plan)
+    check(want, q, c, 0, seqs)
+    for bad in (math.nan, math.inf, -math.inf):
+        c.pool[pages, :, :, :, slots] = bad
+        assert torch.equal(run(way, q, c, 0, seqs, plan), want)
+    c.check()
